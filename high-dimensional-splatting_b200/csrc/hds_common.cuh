@@ -91,6 +91,8 @@ __device__ __forceinline__ bool tile_rect(float u, float v, float a, float b, fl
 // Reads and clears the feature backward kernel's device status (render_features_bwd.cu); the
 // copies are queued on `stream`.
 int read_and_clear_backward_status(int* status, cudaStream_t stream);
+// The same for the codebook lookup's (embedding.cu).
+int read_and_clear_embedding_status(int* status, cudaStream_t stream);
 
 // Lane of the (n+1)-th set bit of mask (n >= 0, fewer than popc(mask)).
 __device__ __forceinline__ int nth_set_bit(unsigned mask, int n) {

@@ -1003,11 +1003,12 @@ extern "C" int hds_render_features_forward(int n, int channels, int width, int h
 extern "C" int hds_device_status(int* status, hds_stream_t stream) {
     clear_error();
     HDS_REQUIRE(status != nullptr, HDS_ERR_INVALID, "device_status: null output");
-    int zero = 0, forward = 0, backward = 0;
+    int zero = 0, forward = 0, backward = 0, embedding = 0;
     HDS_CHECK_CUDA(cudaMemcpyFromSymbolAsync(&forward, g_status, sizeof(int), 0, cudaMemcpyDeviceToHost, stream));
     HDS_CHECK_CUDA(cudaMemcpyToSymbolAsync(g_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream));
     if (int rc = read_and_clear_backward_status(&backward, stream)) return rc;
+    if (int rc = read_and_clear_embedding_status(&embedding, stream)) return rc;
     HDS_CHECK_CUDA(cudaStreamSynchronize(stream));
-    *status = forward ? forward : backward;
+    *status = forward ? forward : (backward ? backward : embedding);
     return HDS_OK;
 }

@@ -1,0 +1,68 @@
+"""Codebook features: the lookup of per-gaussian features in a table, and its gradient.
+
+A compact model holds a codebook [V, C] and one codeword id per gaussian instead of an [N, C] feature
+table.  ``embedding`` gives the [N, C] features that ``rasterize`` blends; its backward sums the blend's
+feature gradient by codeword.  No counterpart in the reference, whose models hold a feature row per
+gaussian.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import gaussian_rasterizer as _ext
+
+
+class Embedding(torch.autograd.Function):
+    """scale * table[ids] with optional dropout; the backward returns dL/dtable in the table's type.
+
+    Under hds_b200.rasterizer.accumulate_leaf_grads() (active during this forward), when table is a leaf
+    that already holds a contiguous float32 .grad of its shape, the backward adds into that buffer and
+    hands autograd no gradient for it (hooks on the table do not see that gradient)."""
+
+    @staticmethod
+    def forward(ctx, table, ids, scale, padding_id, dtype, dropout_p, seed, offset, draw):
+        from . import rasterizer
+
+        ctx.leaf = table if (rasterizer.ACCUMULATE_INTO_LEAF_GRAD and table.is_leaf) else None
+        ctx.table = (table.shape[0], table.dtype)
+        ctx.args = (scale, padding_id, dropout_p, seed, offset)
+        ctx.save_for_backward(ids, draw)
+        return _ext.embedding(table, ids, scale, padding_id, dtype, dropout_p, seed, offset, draw)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        ids, draw = ctx.saved_tensors
+        rows, dtype = ctx.table
+        grad = grad.contiguous()
+        target = ctx.leaf.grad if ctx.leaf is not None else None
+        with torch.cuda.nvtx.range("embedding_backward"):
+            if (target is not None and grad.dtype == torch.float32 and target.dtype == torch.float32
+                    and target.is_contiguous() and target.shape == (rows, grad.shape[-1])
+                    and target.device == grad.device):
+                _ext.embedding_backward_into(target, grad, ids, *ctx.args, draw)
+                return (None,) * 9
+            grad_table = _ext.embedding_backward(grad, ids, rows, dtype, *ctx.args, draw)
+        return (grad_table,) + (None,) * 8
+
+
+def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, padding_id: int | None = None,
+              dtype: torch.dtype | None = None, dropout_p: float = 0.0, seed: int = 0, offset: int = 0,
+              draw: torch.Tensor | None = None) -> torch.Tensor:
+    """scale * table[ids]: the features [*ids.shape, C] of the codeword ids under the codebook table
+    [V, C] (float32, bfloat16 or float16; ids int32 or int64), in `dtype` (the table's type, or float32:
+    the type rasterize takes).  Differentiable in table; the same backward call gives the same bits.
+
+    padding_id: ids with this value (a negative one, say, for gaussians without a codeword) give rows of
+    zeros and no gradient.  Any other id outside [0, V) does too, and sets native.device_status().
+
+    dropout_p: drops elements of the result with this probability (a multiple of 1/65536) and scales the
+    others up, in the same pass.  The mask follows from (seed, offset) -- a step counter, say, as the
+    offset -- and is drawn anew in the backward, never stored.  draw: an int64 tensor [2] = (seed, offset)
+    on the device, used instead of the two numbers and read when the kernels run, so that a captured
+    graph can advance it; it must not change between a forward and its backward."""
+    table = table.contiguous()
+    ids = ids.contiguous()
+    if table.requires_grad and torch.is_grad_enabled():
+        return Embedding.apply(table, ids, scale, padding_id, dtype, dropout_p, seed, offset, draw)
+    return _ext.embedding(table, ids, scale, padding_id, dtype, dropout_p, seed, offset, draw)

@@ -1,0 +1,41 @@
+"""Dropout from a counter-based generator: the mask follows from (seed, offset) alone, is drawn anew by
+the backward, and is never stored.  No counterpart in the reference."""
+from __future__ import annotations
+
+import torch
+
+from . import gaussian_rasterizer as _ext
+
+
+class Dropout(torch.autograd.Function):
+    """y = dropout(x); the backward is the same kernel on dL/dy under the same draw."""
+
+    @staticmethod
+    def forward(ctx, x, p, seed, offset, rows, draw):
+        ctx.args = (p, seed, offset, rows)
+        ctx.save_for_backward(draw)
+        return _ext.dropout(x, p, seed, offset, rows, draw)
+
+    @staticmethod
+    def backward(ctx, grad):
+        (draw,) = ctx.saved_tensors
+        p, seed, offset, rows = ctx.args
+        return dropout(grad, p, seed=seed, offset=offset, rows=rows, draw=draw), None, None, None, None, None
+
+
+def dropout(x: torch.Tensor, p: float, *, seed: int = 0, offset: int = 0, rows: bool = False,
+            draw: torch.Tensor | None = None) -> torch.Tensor:
+    """x (float32, bfloat16 or float16) with each element zeroed with probability p (a multiple of
+    1/65536) and the others scaled by the reciprocal of the kept share.  rows: whole rows along the last
+    dimension are dropped together -- whole gaussians of an [N, C] tensor.
+
+    The mask follows from (seed, offset): another offset, a step counter say, is another mask.  draw: an
+    int64 tensor [2] = (seed, offset) on the device, used instead of the two numbers and read when the
+    kernel runs, so that a captured graph can advance it; it must not change between a forward and its
+    backward.  A p that rounds to 0 returns x itself."""
+    if _ext.drop_threshold(p) == 0:
+        return x
+    x = x.contiguous()
+    if x.requires_grad and torch.is_grad_enabled():
+        return Dropout.apply(x, p, seed, offset, rows, draw)
+    return _ext.dropout(x, p, seed, offset, rows, draw)

@@ -19,7 +19,7 @@ import ctypes
 
 import torch
 
-from .native import check, lib, ptr, stream_of
+from .native import check, lib, on_device, ptr, stream_of
 
 TILE = 16
 _F32 = torch.float32
@@ -449,3 +449,130 @@ def bin_gaussians(means2D, depths, radii, conics, opacities, image_width: int, i
     _, _, values, ranges, keys = _bin(means2D, depths, radii, conics, colors, opacities, int(image_width),
                                       int(image_height), keep_keys=True, origin_y=origin_y)
     return keys, values, ranges
+
+
+# ---------------------------------------------------------------------------------------------
+# codebook features and dropout (no counterpart in the reference)
+# ---------------------------------------------------------------------------------------------
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.int32: 3, torch.int64: 4}
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+_IDS = (torch.int32, torch.int64)
+_DROP_ONE = 65536
+
+
+def drop_threshold(p: float) -> int:
+    """The 16-bit threshold of a dropout probability: an element is dropped with probability
+    round(65536 p) / 65536."""
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout probability must be in [0, 1], got {p}")
+    return round(p * _DROP_ONE)
+
+
+def _draw(seed, offset, draw, device):
+    """(seed, offset, draw pointer): the two numbers modulo 2^64, or the address of an int64 [2] tensor
+    that holds them."""
+    if draw is None:
+        return int(seed) & 0xFFFFFFFFFFFFFFFF, int(offset) & 0xFFFFFFFFFFFFFFFF, None
+    if draw.dtype != torch.int64 or draw.shape != (2,) or not draw.is_contiguous() or draw.device != device:
+        raise RuntimeError("draw must be a contiguous int64 tensor [2] (seed, offset) on the input's device")
+    return 0, 0, draw.data_ptr()
+
+
+def _check_table_ids(table_dtype, value_dtype, ids, device, padding_id):
+    if table_dtype not in _FLOATS or (value_dtype is not table_dtype and value_dtype is not _F32):
+        raise RuntimeError("the table must be float32, bfloat16 or float16, and its values of that type or float32")
+    if ids.dtype not in _IDS:
+        raise RuntimeError("ids must be an int32 or int64 tensor")
+    if ids.device != device:
+        raise RuntimeError("ids must be on the table's device")
+    if not ids.is_contiguous():
+        raise RuntimeError("ids must be contiguous")
+    if padding_id is not None and not -2**63 <= padding_id < 2**63:
+        raise ValueError(f"padding_id {padding_id} does not fit 64 bits")
+
+
+def embedding(table, ids, scale: float = 1.0, padding_id: int | None = None, dtype=None, dropout_p: float = 0.0,
+              seed: int = 0, offset: int = 0, draw=None):
+    """scale * table[ids], with dropout of its elements in the same pass.  table [V, C] float32, bfloat16
+    or float16; ids any shape, int32 or int64.  Returns [*ids.shape, C] of `dtype` (the table's type, the
+    default, or float32).
+
+    An id equal to padding_id gives a row of zeros.  So does any other id outside [0, V), which also sets
+    the device status word (native.device_status).  The dropout mask is drawn from (seed, offset), or from
+    the int64 tensor draw = [seed, offset] read on the device when the kernel runs (for captured graphs);
+    hds_b200.h defines it."""
+    _check(table, "table")
+    if table.dim() != 2:
+        raise RuntimeError("table must be [V, C]")
+    dtype = dtype or table.dtype
+    dev = table.device
+    _check_table_ids(table.dtype, dtype, ids, dev, padding_id)
+    threshold = drop_threshold(dropout_p)
+    seed, offset, draw_ptr = _draw(seed, offset, draw, dev)
+    v, c = table.shape
+    out = torch.empty(*ids.shape, c, dtype=dtype, device=dev)
+    with on_device(dev):
+        check(lib.hds_embedding_forward(ids.numel(), v, c, _TYPES[table.dtype], table.data_ptr(), _TYPES[ids.dtype],
+                                        ids.data_ptr(), padding_id is not None, padding_id or 0, scale, threshold,
+                                        seed, offset, draw_ptr, _TYPES[dtype], out.data_ptr(), stream_of(dev)))
+    return out
+
+
+def _embedding_backward(grad, ids, grad_table, accumulate, scale, padding_id, dropout_p, seed, offset, draw):
+    dev = grad_table.device
+    _check(grad, "grad")
+    v, c = grad_table.shape
+    if grad.device != dev or grad.shape != (*ids.shape, c):
+        raise RuntimeError(f"grad must be {(*ids.shape, c)} on the table's device")
+    _check_table_ids(grad_table.dtype, grad.dtype, ids, dev, padding_id)
+    threshold = drop_threshold(dropout_p)
+    seed, offset, draw_ptr = _draw(seed, offset, draw, dev)
+    n = ids.numel()
+    scratch = torch.empty(lib.hds_embedding_backward_scratch_bytes(n, v, c), dtype=torch.uint8, device=dev)
+    with on_device(dev):
+        check(lib.hds_embedding_backward(n, v, c, _TYPES[grad.dtype], grad.data_ptr(), _TYPES[ids.dtype],
+                                         ids.data_ptr(), padding_id is not None, padding_id or 0, scale, threshold,
+                                         seed, offset, draw_ptr, _TYPES[grad_table.dtype], grad_table.data_ptr(),
+                                         accumulate, scratch.data_ptr(), scratch.numel(), stream_of(dev)))
+
+
+def embedding_backward(grad, ids, rows: int, dtype=None, scale: float = 1.0, padding_id: int | None = None,
+                       dropout_p: float = 0.0, seed: int = 0, offset: int = 0, draw=None):
+    """dL/dtable [rows, C] (`dtype`: grad's by default) of embedding() with the same arguments: scale *
+    the sum of grad's kept elements over the rows of each id, in fp32.  The same call gives the same bits."""
+    grad_table = torch.empty(int(rows), grad.shape[-1], dtype=dtype or grad.dtype, device=grad.device)
+    _embedding_backward(grad, ids, grad_table, 0, scale, padding_id, dropout_p, seed, offset, draw)
+    return grad_table
+
+
+def embedding_backward_into(grad_table, grad, ids, scale: float = 1.0, padding_id: int | None = None,
+                            dropout_p: float = 0.0, seed: int = 0, offset: int = 0, draw=None):
+    """embedding_backward that ADDS into grad_table ([V, C] float32, contiguous).  Rows whose id does not
+    occur are left as they are."""
+    if not (grad_table.is_cuda and grad_table.dim() == 2 and grad_table.is_contiguous() and grad_table.dtype == _F32):
+        raise RuntimeError("grad_table must be a contiguous float32 CUDA tensor [V, C]")
+    if grad.dtype != _F32:
+        raise RuntimeError("grad must be float32 to be added into a float32 table gradient")
+    _embedding_backward(grad, ids, grad_table, 1, scale, padding_id, dropout_p, seed, offset, draw)
+
+
+def dropout(x, p: float, seed: int = 0, offset: int = 0, rows: bool = False, draw=None):
+    """x with elements (rows: whole rows along the last dimension) zeroed with probability p and the others
+    scaled by the reciprocal of the kept share.  float32, bfloat16 or float16, contiguous.  The mask is
+    drawn from (seed, offset), as in embedding(), and never stored: the gradient is the same call on dL/dy."""
+    _check(x, "x")
+    if x.dtype not in _FLOATS:
+        raise RuntimeError("x must be float32, bfloat16 or float16")
+    if rows and x.dim() == 0:
+        raise RuntimeError("dropping whole rows needs at least one dimension")
+    threshold = drop_threshold(p)
+    dev = x.device
+    seed, offset, draw_ptr = _draw(seed, offset, draw, dev)
+    y = torch.empty_like(x)
+    n = x.numel()
+    c = x.shape[-1] if rows else 1
+    with on_device(dev):
+        check(lib.hds_dropout(n // c if c else 0, c, _TYPES[x.dtype], x.data_ptr(), threshold, bool(rows), seed, offset,
+                              draw_ptr, y.data_ptr(), stream_of(dev)))
+    return y

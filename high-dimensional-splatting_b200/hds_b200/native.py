@@ -7,8 +7,9 @@ it with ``python high-dimensional-splatting_b200/build.py``.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
-from ctypes import c_float, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_double, c_float, c_int, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libhds_b200.so"
@@ -56,6 +57,12 @@ SIGNATURES = {
     "hds_densify_stats": [c_int, P, P, c_int, c_int, P, P, P, S],
     "hds_densify_apply": [c_int, c_int, c_int, ctypes.POINTER(c_int), c_int, c_int, c_float, P, P, P, P, P, P, P, P,
                           P, S],
+    "hds_embedding_forward": [c_int64, c_int64, c_int, c_int, P, c_int, P, c_int, c_int64, c_double, c_int, c_uint64,
+                              c_uint64, P, c_int, P, S],
+    "hds_embedding_backward_scratch_bytes": [c_int64, c_int64, c_int],
+    "hds_embedding_backward": [c_int64, c_int64, c_int, c_int, P, c_int, P, c_int, c_int64, c_double, c_int, c_uint64,
+                               c_uint64, P, c_int, P, c_int, P, c_size_t, S],
+    "hds_dropout": [c_int64, c_int64, c_int, P, c_int, c_int, c_uint64, c_uint64, P, P, S],
     "hds_device_status": [ctypes.POINTER(c_int), S],
     "hds_rasterize_bin_noalloc": [c_int, P, P, P, P, P, P, c_int, c_int, P, P, P, c_int64, P,
                                   ctypes.POINTER(c_int64), S],
@@ -67,6 +74,7 @@ RESTYPES = {
     "hds_rasterize_prepare_scratch_bytes": c_size_t,
     "hds_rasterize_sort_scratch_bytes": c_size_t,
     "hds_backward_workspace_bytes": c_size_t,
+    "hds_embedding_backward_scratch_bytes": c_size_t,
     "hds_last_error": ctypes.c_char_p,
     "hds_launch_count": ctypes.c_ulonglong,
 }
@@ -123,8 +131,18 @@ def stream_of(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def on_device(device):
+    """Context in which `device` is the current CUDA device (the C ABI launches on the current one)."""
+    import torch
+
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
 def device_status(device=None) -> int:
-    """Reads and clears the device-side failure word (0 = no bounded wait ran out)."""
+    """Reads and clears the device-side failure word (0 = no bounded wait ran out and no codebook id lay
+    outside its table)."""
     out = c_int(0)
     check(lib.hds_device_status(ctypes.byref(out), stream_of(device)))
     return out.value

@@ -301,8 +301,59 @@ int hds_densify_apply(int n_old, int n_new, int segments, const int* widths, int
                       const float* old_params, const float* old_exp_avg, const float* old_exp_avg_sq, float* new_params,
                       float* new_exp_avg, float* new_exp_avg_sq, hds_stream_t stream);
 
-/* Reads and clears the device-side failure word that kernels with bounded waits set (0 = none).
- * Synchronises `stream`. */
+/* ---------------------------------------------------------------------------------------------
+ * Codebook features.  No counterpart in the reference: its models hold one feature row per gaussian.
+ * A compact model holds a codebook table [vocab, channels] and one id per gaussian; the lookup gives
+ * the feature rows [n, channels] that the feature blend takes.
+ *
+ * Element types: HDS_TYPE_F32, HDS_TYPE_BF16, HDS_TYPE_F16; ids HDS_TYPE_I32 or HDS_TYPE_I64.  The
+ * looked-up values (and their gradient) are of the table's type or fp32.  Arithmetic is fp32, rounded
+ * once when stored.  Pointers need the alignment of their elements only; 32-byte aligned buffers with
+ * channels a multiple of 8 move as vectors.
+ *
+ * Dropout (both directions of the lookup, and hds_dropout): drop_threshold T in [0, 65536] drops an
+ * element with probability T / 65536 and scales the others by 65536 / (65536 - T); 0 is no dropout.
+ * The mask is never stored: every call draws it anew from (seed, offset).  Element e (row-major in the
+ * [n, channels] values) takes half e % 8, low half first, of the four words that Philox4x32-10 gives
+ * for the counter words (lo(e / 8), hi(e / 8), lo(offset), hi(offset)) and the key (lo(seed), hi(seed)),
+ * and is dropped when that 16-bit number is below T.  draw, when not NULL, is {seed, offset} in device
+ * memory (8-byte aligned), read when the kernels run instead of the two arguments, so that a captured
+ * graph can take a new mask at every replay.  Dropped elements are 0 whatever the input holds.
+ *
+ * hds_embedding_forward: out[i] = scale * table[ids[i]] [n, channels].  An id equal to padding_id (when
+ * has_padding) gives a row of zeros and takes no gradient.  So does any other id outside [0, vocab),
+ * which also records HDS_ERR_INVALID in the device status (hds_device_status).
+ *
+ * hds_embedding_backward: grad_table[v] = scale * sum of grad[i] over the i with ids[i] = v, in fp32 and
+ * in an order that depends on the arguments alone: the same call gives the same bits.  accumulate != 0
+ * (fp32 tables) adds it to what grad_table holds and leaves the rows of absent ids untouched; 0 writes
+ * every row.  scratch: hds_embedding_backward_scratch_bytes(n, vocab, channels) bytes, 256-byte aligned.
+ *
+ * hds_dropout: y = dropout(x), x and y [rows, channels] of one type; y may be x.  whole_rows drops whole
+ * rows (e above is the row).  The gradient is the same call on dL/dy with the same draw.
+ * ------------------------------------------------------------------------------------------- */
+enum {
+    HDS_TYPE_F32 = 0,
+    HDS_TYPE_BF16 = 1,
+    HDS_TYPE_F16 = 2,
+    HDS_TYPE_I32 = 3,
+    HDS_TYPE_I64 = 4
+};
+#define HDS_EMBEDDING_MAX_CHANNELS 32768
+int hds_embedding_forward(int64_t n, int64_t vocab, int channels, int table_type, const void* table, int ids_type,
+                          const void* ids, int has_padding, int64_t padding_id, double scale, int drop_threshold,
+                          uint64_t seed, uint64_t offset, const int64_t* draw, int out_type, void* out,
+                          hds_stream_t stream);
+size_t hds_embedding_backward_scratch_bytes(int64_t n, int64_t vocab, int channels);
+int hds_embedding_backward(int64_t n, int64_t vocab, int channels, int grad_type, const void* grad, int ids_type,
+                           const void* ids, int has_padding, int64_t padding_id, double scale, int drop_threshold,
+                           uint64_t seed, uint64_t offset, const int64_t* draw, int table_type, void* grad_table,
+                           int accumulate, void* scratch, size_t scratch_bytes, hds_stream_t stream);
+int hds_dropout(int64_t rows, int64_t channels, int type, const void* x, int drop_threshold, int whole_rows,
+                uint64_t seed, uint64_t offset, const int64_t* draw, void* y, hds_stream_t stream);
+
+/* Reads and clears the device-side failure word that kernels with bounded waits and the codebook lookup
+ * set (0 = none).  Synchronises `stream`. */
 int hds_device_status(int* status, hds_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------

@@ -31,9 +31,7 @@ struct Padding {
 };
 
 // The table row of an id, or -1 for a row of zeros (padding, or outside the table: recorded).
-template <typename I>
-__device__ __forceinline__ int64_t table_row(I id, int64_t vocab, const Padding& padding) {
-    const int64_t v = (int64_t)id;
+__device__ __forceinline__ int64_t table_row(int64_t v, int64_t vocab, const Padding& padding) {
     if (padding.present && v == padding.id) return -1;
     if (v < 0 || v >= vocab) {
         atomicExch(&g_embedding_status, HDS_ERR_INVALID);
@@ -44,18 +42,72 @@ __device__ __forceinline__ int64_t table_row(I id, int64_t vocab, const Padding&
 
 constexpr int THREADS = 256;
 
-template <typename T, typename O, typename I>
-__global__ void __launch_bounds__(THREADS) lookup_kernel(int64_t n, int64_t vocab, int channels,
-                                                         const T* __restrict__ table, const I* __restrict__ ids,
-                                                         Padding padding, float factor, uint32_t threshold, Draw draw,
+// ---------------------------------------------------------------------------------------------
+// lookup
+// ---------------------------------------------------------------------------------------------
+// A warp writes tiles of 256 consecutive output elements in vectors of V, the widest into which rows
+// split and to which both buffers are aligned.  All of a warp's ids are loaded first, then all of its
+// table vectors, then it stores: TILES x 8 elements in flight per lane cover the two dependent loads.
+// Dropout: lane j draws group j of the tile, the holder of an element fetches its group's decisions with
+// a shuffle (itself when V = 8).
+constexpr int TILE_ELEMENTS = 256;
+constexpr int TILES = 4;
+constexpr int LOOKUP_ELEMENTS = THREADS / 32 * TILE_ELEMENTS * TILES;  // per block
+
+struct Ids {
+    const void* p;
+    int wide;  // int64 (else int32)
+    __device__ __forceinline__ int64_t operator[](int64_t i) const {
+        return wide ? __ldg(static_cast<const long long*>(p) + i) : (int64_t)__ldg(static_cast<const int*>(p) + i);
+    }
+};
+
+template <typename T, typename O, int V, bool DROP>
+__global__ void __launch_bounds__(THREADS) lookup_kernel(int64_t total, int64_t vocab, int channels, Divider rows_of,
+                                                         const T* __restrict__ table, Ids ids, Padding padding,
+                                                         float factor, uint32_t threshold, Draw draw,
                                                          O* __restrict__ out) {
-    draw = resolve(draw);
-    const int64_t total = n * channels, stride = (int64_t)gridDim.x * blockDim.x;
-    for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += stride) {
-        const int64_t i = e / channels;
-        const int64_t row = table_row(ids[i], vocab, padding);
-        const bool keep = row >= 0 && (threshold == 0 || keep_one((uint64_t)e, draw, threshold));
-        out[e] = from_float<O>(keep ? to_float(table[row * channels + (e - i * channels)]) * factor : 0.0f);
+    constexpr int STEPS = 8 / V;
+    if (DROP) draw = resolve(draw);
+    const int lane = threadIdx.x & 31;
+    const int64_t warp_base = (int64_t)blockIdx.x * LOOKUP_ELEMENTS + (threadIdx.x >> 5) * (TILE_ELEMENTS * TILES);
+    if (warp_base >= total) return;
+    const int64_t row0 = warp_base / channels;
+    const uint32_t place = (uint32_t)(warp_base - row0 * channels);
+    int64_t at[TILES][STEPS];  // the vector's first element in the table, or -1
+#pragma unroll
+    for (int t = 0; t < TILES; t++)
+#pragma unroll
+        for (int k = 0; k < STEPS; k++) {
+            const uint32_t e = t * TILE_ELEMENTS + (k * 32 + lane) * V;
+            at[t][k] = -1;
+            if (warp_base + e < total) {
+                const uint32_t q = rows_of.quotient(place + e);
+                const int64_t row = table_row(ids[row0 + q], vocab, padding);
+                if (row >= 0) at[t][k] = row * channels + (place + e - q * channels);
+            }
+        }
+    Vec<T, V> v[TILES][STEPS];
+#pragma unroll
+    for (int t = 0; t < TILES; t++)
+#pragma unroll
+        for (int k = 0; k < STEPS; k++)
+            if (at[t][k] >= 0) v[t][k] = load_shared_data<T, V>(table + at[t][k]);
+#pragma unroll
+    for (int t = 0; t < TILES; t++) {
+        const int64_t tile = warp_base + t * TILE_ELEMENTS;
+        const uint32_t bits = DROP ? keep8((uint64_t)(tile >> 3) + lane, draw, threshold) : 0xffu;
+#pragma unroll
+        for (int k = 0; k < STEPS; k++) {
+            const int e = (k * 32 + lane) * V;
+            uint32_t keep = bits;
+            if (DROP && V < 8) keep = __shfl_sync(FULL_MASK, bits, e >> 3) >> (e & 7);
+            if (at[t][k] < 0) keep = 0;
+            Vec<O, V> r;
+#pragma unroll
+            for (int j = 0; j < V; j++) r.set(j, (keep >> j) & 1u ? v[t][k].get(j) * factor : 0.0f);
+            if (tile + e < total) store<O, V>(out + tile + e, r);
+        }
     }
 }
 
@@ -265,20 +317,28 @@ extern "C" int hds_embedding_forward(int64_t n, int64_t vocab, int channels, int
     const Padding padding{has_padding, padding_id};
     const Draw d{seed, offset, draw};
     const float factor = keep_factor(scale, drop_threshold);
-    const int64_t blocks = std::min<int64_t>((n * channels + THREADS - 1) / THREADS, 148 * 8);
+    const int64_t total = n * channels;
+    const int64_t blocks = (total + LOOKUP_ELEMENTS - 1) / LOOKUP_ELEMENTS;
+    HDS_REQUIRE(blocks <= INT32_MAX, HDS_ERR_TOO_LARGE, "embedding: n = %lld, channels = %d is too large",
+                (long long)n, channels);
+    const Ids id{ids, ids_type == HDS_TYPE_I64};
+    const Divider rows_of = divider((uint32_t)channels);
     return with_types(table_type, out_type, [&](auto t, auto o) -> int {
         using T = decltype(t);
         using O = decltype(o);
-        if (ids_type == HDS_TYPE_I32)
-            lookup_kernel<T, O, int32_t><<<(unsigned)blocks, THREADS, 0, stream>>>(
-                n, vocab, channels, static_cast<const T*>(table), static_cast<const int32_t*>(ids), padding, factor,
-                (uint32_t)drop_threshold, d, static_cast<O*>(out));
-        else
-            lookup_kernel<T, O, int64_t><<<(unsigned)blocks, THREADS, 0, stream>>>(
-                n, vocab, channels, static_cast<const T*>(table), static_cast<const int64_t*>(ids), padding, factor,
-                (uint32_t)drop_threshold, d, static_cast<O*>(out));
-        HDS_CHECK_LAUNCH("lookup_kernel");
-        return HDS_OK;
+        return with_vector(widest_vector(channels, {{table, table_type}, {out, out_type}}), [&](auto width) -> int {
+            constexpr int V = decltype(width)::value;
+            if (drop_threshold > 0)
+                lookup_kernel<T, O, V, true><<<(unsigned)blocks, THREADS, 0, stream>>>(
+                    total, vocab, channels, rows_of, static_cast<const T*>(table), id, padding, factor,
+                    (uint32_t)drop_threshold, d, static_cast<O*>(out));
+            else
+                lookup_kernel<T, O, V, false><<<(unsigned)blocks, THREADS, 0, stream>>>(
+                    total, vocab, channels, rows_of, static_cast<const T*>(table), id, padding, factor, 0u, d,
+                    static_cast<O*>(out));
+            HDS_CHECK_LAUNCH("lookup_kernel");
+            return HDS_OK;
+        });
     });
 }
 

@@ -8,81 +8,129 @@
 namespace hds {
 namespace {
 
-// A warp takes tiles of 256 consecutive elements: lane j draws the eight decisions of group j of the tile
-// (one generator call for eight elements, whatever the vector width), and the lane that holds an
-// element fetches its group's decisions with a shuffle.  With 8-element vectors that is the lane itself.
-// Whole rows: lane j draws for the rows 8 (r0 / 8 + j) .. + 7 around the tile's first row r0; a tile
-// of rows at least two wide spans at most 18 such groups.  A dropped row is not read.
+// A warp takes tiles of 256 consecutive elements in vectors of V (8 unless a buffer is aligned to less;
+// rows need not be whole vectors).
+//
+// Elements: lane j draws the eight decisions of group j of the tile, one generator call for eight elements
+// whatever V is, and the lane that holds an element fetches its group's decisions with a shuffle; with
+// 8-element vectors that is the lane itself.
+//
+// Whole rows: lane j draws for the rows 8 (r0 / 8 + j) .. + 7 around the tile's first row r0; a tile of rows
+// at least two wide spans at most 18 such groups.  Of rows at least V wide a vector meets two at most.
+// A vector all of whose rows are dropped is not read.
 constexpr int DROPOUT_THREADS = 256;
 constexpr int TILE_ELEMENTS = 256;  // per warp
 constexpr int TILES = 4;            // tiles in flight per warp
 constexpr int BLOCK_ELEMENTS = DROPOUT_THREADS / 32 * TILE_ELEMENTS * TILES;
+constexpr int BLOCK_GROUPS = BLOCK_ELEMENTS / 8;
 
-template <typename T, int V, bool ROWS>
-__global__ void __launch_bounds__(DROPOUT_THREADS) dropout_kernel(int64_t n, int64_t row_width, Divider rows_of,
-                                                                  const T* x, float factor, uint32_t threshold,
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> load_up_to(const T* x, int64_t e, int64_t n) {
+    if (e + V <= n) return load_once<T, V>(x + e);
+    Vec<T, V> v;
+    for (int j = 0; j < V; j++) v.set(j, e + j < n ? to_float(x[e + j]) : 0.0f);
+    return v;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_up_to(T* y, int64_t e, int64_t n, const Vec<T, V>& v) {
+    if (e + V <= n)
+        store<T, V>(y + e, v);
+    else
+        for (int j = 0; j < V; j++)
+            if (e + j < n) y[e + j] = from_float<T>(v.get(j));
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(DROPOUT_THREADS) dropout_kernel(int64_t n, const T* x, float factor, uint32_t last,
                                                                   Draw draw, T* y) {
+    constexpr int STEPS = 8 / V;
+    draw = resolve(draw);
+    const int lane = threadIdx.x & 31;
+    const int in_block = (threadIdx.x >> 5) * (TILE_ELEMENTS * TILES);
+    const int64_t warp_base = (int64_t)blockIdx.x * BLOCK_ELEMENTS + in_block;
+    // A block's groups share the upper counter word: its first is a multiple of their number.
+    const uint64_t group0 = (uint64_t)blockIdx.x * BLOCK_GROUPS;
+    Vec<T, V> v[TILES][STEPS];
+#pragma unroll
+    for (int t = 0; t < TILES; t++)
+#pragma unroll
+        for (int k = 0; k < STEPS; k++)
+            v[t][k] = load_up_to<T, V>(x, warp_base + t * TILE_ELEMENTS + (k * 32 + lane) * V, n);
+#pragma unroll
+    for (int t = 0; t < TILES; t++) {
+        const Numbers8 numbers = philox4x32_10((uint32_t)group0 + (in_block + t * TILE_ELEMENTS) / 8 + lane,
+                                               (uint32_t)(group0 >> 32), draw);
+        const uint32_t bits = V == 8 ? 0 : numbers.bits(last);
+#pragma unroll
+        for (int k = 0; k < STEPS; k++) {
+            const int at = (k * 32 + lane) * V;
+            const uint32_t mine = V == 8 ? 0 : __shfl_sync(FULL_MASK, bits, at >> 3) >> (at & 7);
+            Vec<T, V> r;
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                const bool kept = V == 8 ? numbers.kept(j, last) : ((mine >> j) & 1u) != 0;
+                r.set(j, kept ? v[t][k].get(j) * factor : 0.0f);
+            }
+            store_up_to<T, V>(y, warp_base + t * TILE_ELEMENTS + at, n, r);
+        }
+    }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(DROPOUT_THREADS) dropout_rows_kernel(int64_t n, int64_t row_width, Divider rows_of,
+                                                                       const T* x, float factor, uint32_t last,
+                                                                       Draw draw, T* y) {
     constexpr int STEPS = 8 / V;
     draw = resolve(draw);
     const int lane = threadIdx.x & 31;
     const int64_t warp_base =
         (int64_t)blockIdx.x * BLOCK_ELEMENTS + (threadIdx.x >> 5) * (TILE_ELEMENTS * TILES);
-    const int64_t row0 = ROWS ? warp_base / row_width : 0;  // the warp's first element's row,
-    const int64_t place = warp_base - row0 * row_width;     // and its place in it
+    const int64_t row0 = warp_base / row_width;          // the warp's first element's row,
+    const int64_t place = warp_base - row0 * row_width;  // and its place in it
+    // Rows from row0 to the row of an element `at` elements from the warp's first.
+    const auto rows_on = [&](uint32_t at) -> uint32_t {
+        if (rows_of.d != 0) return rows_of.quotient((uint32_t)place + at);
+        return place + at >= row_width ? 1 : 0;
+    };
     Vec<T, V> v[TILES][STEPS];
     uint32_t keep[TILES][STEPS];
-    if (!ROWS) {
-#pragma unroll
-        for (int t = 0; t < TILES; t++)
-#pragma unroll
-            for (int k = 0; k < STEPS; k++) {
-                const int64_t e = warp_base + t * TILE_ELEMENTS + (k * 32 + lane) * V;
-                if (e + V <= n)
-                    v[t][k] = load_once<T, V>(x + e);
-                else
-                    for (int j = 0; j < V; j++) v[t][k].set(j, e + j < n ? to_float(x[e + j]) : 0.0f);
-            }
-    }
 #pragma unroll
     for (int t = 0; t < TILES; t++) {
-        const int64_t tile = warp_base + t * TILE_ELEMENTS;
-        if (!ROWS) {
-            const uint32_t bits = keep8((uint64_t)(tile >> 3) + lane, draw, threshold);
+        const int64_t group0 = (row0 + rows_on(t * TILE_ELEMENTS)) >> 3;
+        const uint32_t bits = philox4x32_10((uint64_t)(group0 + lane), draw).bits(last);
+        const int first = (int)(row0 - 8 * group0);  // of row0 among the tile's decisions
+        const auto row_kept = [&](uint32_t on) -> uint32_t {  // the row `on` rows from row0
+            const int bit = first + (int)on;
+            return (__shfl_sync(FULL_MASK, bits, bit >> 3) >> (bit & 7)) & 1u;
+        };
 #pragma unroll
-            for (int k = 0; k < STEPS; k++) {
-                const int at = (k * 32 + lane) * V;
-                keep[t][k] = V == 8 ? bits : __shfl_sync(FULL_MASK, bits, at >> 3) >> (at & 7);
-            }
-        } else {
-            const auto row_of = [&](uint32_t at) -> int64_t {  // at: elements from the warp's first
-                if (rows_of.d != 0) return row0 + rows_of.quotient((uint32_t)place + at);
-                return row0 + (place + at >= row_width ? 1 : 0);
-            };
-            const int64_t group0 = row_of(t * TILE_ELEMENTS) >> 3;
-            const uint32_t bits = keep8((uint64_t)(group0 + lane), draw, threshold);
+        for (int k = 0; k < STEPS; k++) {
+            const uint32_t at = t * TILE_ELEMENTS + (k * 32 + lane) * V;
+            uint32_t mine = 0;
+            if (V > 1 && row_width < V) {
 #pragma unroll
-            for (int k = 0; k < STEPS; k++) {
-                const int at = t * TILE_ELEMENTS + (k * 32 + lane) * V;
-                const int64_t row = row_of(at);
-                const uint32_t mine = __shfl_sync(FULL_MASK, bits, (int)((row >> 3) - group0));
-                keep[t][k] = (mine >> (row & 7)) & 1u ? 0xffu : 0u;
-                if (keep[t][k] && warp_base + at < n) v[t][k] = load_once<T, V>(x + warp_base + at);
+                for (int j = 0; j < V; j++) mine |= row_kept(rows_on(at + j)) << j;
+            } else {
+                const uint32_t on = rows_on(at), on_end = rows_on(at + V - 1);
+                const uint32_t a = row_kept(on), b = row_kept(on_end);
+                // Elements of the vector in its first row.
+                const int64_t left = (int64_t)(on + 1) * row_width - place - at;
+                const uint32_t low = left >= V ? (1u << V) - 1u : (1u << (int)left) - 1u;
+                mine = (a ? low : 0u) | (b ? ((1u << V) - 1u) & ~low : 0u);
             }
+            keep[t][k] = mine;
+            if (mine != 0) v[t][k] = load_up_to<T, V>(x, warp_base + at, n);
         }
     }
 #pragma unroll
     for (int t = 0; t < TILES; t++)
 #pragma unroll
         for (int k = 0; k < STEPS; k++) {
-            const int64_t e = warp_base + t * TILE_ELEMENTS + (k * 32 + lane) * V;
             Vec<T, V> r;
 #pragma unroll
             for (int j = 0; j < V; j++) r.set(j, (keep[t][k] >> j) & 1u ? v[t][k].get(j) * factor : 0.0f);
-            if (e + V <= n)
-                store<T, V>(y + e, r);
-            else
-                for (int j = 0; j < V; j++)
-                    if (e + j < n) y[e + j] = from_float<T>(r.get(j));
+            store_up_to<T, V>(y, warp_base + t * TILE_ELEMENTS + (k * 32 + lane) * V, n, r);
         }
 }
 
@@ -106,29 +154,31 @@ extern "C" int hds_dropout(int64_t rows, int64_t channels, int type, const void*
     HDS_REQUIRE((((uintptr_t)x | (uintptr_t)y) & (element_size(type) - 1)) == 0 && ((uintptr_t)draw & 7) == 0,
                 HDS_ERR_INVALID, "dropout: misaligned buffer");
     const int64_t n = rows * channels;
+    if (drop_threshold == 0) {
+        if (x != y)
+            HDS_CHECK_CUDA(cudaMemcpyAsync(y, x, (size_t)n * element_size(type), cudaMemcpyDeviceToDevice, stream));
+        return HDS_OK;
+    }
     const float factor = keep_factor(1.0, drop_threshold);
     const Draw d{seed, offset, draw};
-    // Rows of one element are elements.  Element by element, vectors need not end with a row: only the
-    // alignment bounds them, and the last n % V elements go one by one.
-    const bool by_rows = whole_rows && channels > 1;
-    const int v = widest_vector(by_rows ? channels : 8, {{x, type}, {y, type}});
+    const int v = widest_vector(8, {{x, type}, {y, type}});
     const int64_t blocks = (n + BLOCK_ELEMENTS - 1) / BLOCK_ELEMENTS;
     HDS_REQUIRE(blocks <= INT32_MAX, HDS_ERR_TOO_LARGE, "dropout: [%lld, %lld] is too large", (long long)rows,
                 (long long)channels);
-    // d = 0: rows of 2^15 elements and more, found by comparing (a warp's 1024 elements span two at most).
+    const uint32_t last = below_last(drop_threshold);
+    // d = 0: rows of 2^15 elements and more, found by comparing (a warp's 1024 elements meet two at most).
     const Divider rows_of = channels < (1 << 15) ? divider((uint32_t)channels) : Divider{0, 0};
     return with_type(type, [&](auto t) -> int {
         using T = decltype(t);
+        const T* from = static_cast<const T*>(x);
+        T* to = static_cast<T*>(y);
         return with_vector(v, [&](auto width) -> int {
             constexpr int V = decltype(width)::value;
-            if (by_rows)
-                dropout_kernel<T, V, true><<<(unsigned)blocks, DROPOUT_THREADS, 0, stream>>>(
-                    n, channels, rows_of, static_cast<const T*>(x), factor, (uint32_t)drop_threshold, d,
-                    static_cast<T*>(y));
+            if (whole_rows && channels > 1)  // a row of one element is an element
+                dropout_rows_kernel<T, V><<<(unsigned)blocks, DROPOUT_THREADS, 0, stream>>>(n, channels, rows_of, from,
+                                                                                           factor, last, d, to);
             else
-                dropout_kernel<T, V, false><<<(unsigned)blocks, DROPOUT_THREADS, 0, stream>>>(
-                    n, 1, Divider{0, 0}, static_cast<const T*>(x), factor, (uint32_t)drop_threshold, d,
-                    static_cast<T*>(y));
+                dropout_kernel<T, V><<<(unsigned)blocks, DROPOUT_THREADS, 0, stream>>>(n, from, factor, last, d, to);
             HDS_CHECK_LAUNCH("dropout_kernel");
             return HDS_OK;
         });

@@ -23,16 +23,39 @@ struct Draw {
     const int64_t* device;  // {seed, offset}, or NULL
 };
 
+// The draw as numbers that are the same in every lane: the reductions tell the compiler so, which then
+// keeps the ten round keys and what the offset alone decides out of the lanes' integer work.  Every lane
+// of the warp must call it.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __reduce_or_sync(FULL_MASK, x); }
+
 __device__ __forceinline__ Draw resolve(Draw d) {
     if (d.device != nullptr) {
         d.seed = (uint64_t)d.device[0];
         d.offset = (uint64_t)d.device[1];
     }
+    d.seed = (uint64_t)uniform((uint32_t)(d.seed >> 32)) << 32 | uniform((uint32_t)d.seed);
+    d.offset = (uint64_t)uniform((uint32_t)(d.offset >> 32)) << 32 | uniform((uint32_t)d.offset);
     return d;
 }
 
-__device__ __forceinline__ uint4 philox4x32_10(uint64_t counter, const Draw& d) {
-    uint32_t x0 = (uint32_t)counter, x1 = (uint32_t)(counter >> 32);
+// The eight 16-bit numbers of a group: number j is the low (j even) or high half of word j / 2.
+struct Numbers8 {
+    uint32_t w[4];
+    // below_last = 65536 T - 1: a number is >= T when, moved to the upper half of a word, it is greater.
+    __device__ __forceinline__ bool kept(int j, uint32_t below_last) const {
+        return (j % 2 == 0 ? w[j / 2] << 16 : w[j / 2]) > below_last;
+    }
+    // Bit j: whether number j is kept.
+    __device__ __forceinline__ uint32_t bits(uint32_t below_last) const {
+        uint32_t b = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) b |= kept(j, below_last) ? 1u << j : 0u;
+        return b;
+    }
+};
+
+__device__ __forceinline__ Numbers8 philox4x32_10(uint32_t group_low, uint32_t group_high, const Draw& d) {
+    uint32_t x0 = group_low, x1 = group_high;
     uint32_t x2 = (uint32_t)d.offset, x3 = (uint32_t)(d.offset >> 32);
     uint32_t k0 = (uint32_t)d.seed, k1 = (uint32_t)(d.seed >> 32);
 #pragma unroll
@@ -45,25 +68,15 @@ __device__ __forceinline__ uint4 philox4x32_10(uint64_t counter, const Draw& d) 
         k0 += 0x9E3779B9u;
         k1 += 0xBB67AE85u;
     }
-    return make_uint4(x0, x1, x2, x3);
+    return Numbers8{{x0, x1, x2, x3}};
 }
 
-// Bit j: whether element 8 group + j is kept.
-__device__ __forceinline__ uint32_t keep8(uint64_t group, const Draw& d, uint32_t threshold) {
-    const uint4 w = philox4x32_10(group, d);
-    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-    uint32_t bits = 0;
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        bits |= ((words[k] & 0xffffu) >= threshold ? 1u : 0u) << (2 * k);
-        bits |= ((words[k] >> 16) >= threshold ? 2u : 0u) << (2 * k);
-    }
-    return bits;
+__device__ __forceinline__ Numbers8 philox4x32_10(uint64_t group, const Draw& d) {
+    return philox4x32_10((uint32_t)group, (uint32_t)(group >> 32), d);
 }
 
-__device__ __forceinline__ bool keep_one(uint64_t e, const Draw& d, uint32_t threshold) {
-    return (keep8(e >> 3, d, threshold) >> (e & 7)) & 1u;
-}
+// For the kernels' below_last; thresholds from 1 to 65536 (modulo 2^32).
+inline uint32_t below_last(int threshold) { return (uint32_t)((uint64_t)threshold * 65536u - 1u); }
 
 // scale / (the kept share), rounded once to float; 0 when everything is dropped.
 inline float keep_factor(double scale, int threshold) {

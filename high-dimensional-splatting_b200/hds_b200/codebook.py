@@ -10,6 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import gaussian_rasterizer as _ext
+from . import rasterizer
 
 
 class Embedding(torch.autograd.Function):
@@ -20,30 +21,28 @@ class Embedding(torch.autograd.Function):
     hands autograd no gradient for it (hooks on the table do not see that gradient)."""
 
     @staticmethod
-    def forward(ctx, table, ids, scale, padding_id, dtype, dropout_p, seed, offset, draw):
-        from . import rasterizer
-
+    def forward(ctx, table, ids, dtype, how):
+        """how: embedding()'s (scale, padding_id, dropout_p, seed, offset, draw)."""
         ctx.leaf = table if (rasterizer.ACCUMULATE_INTO_LEAF_GRAD and table.is_leaf) else None
         ctx.table = (table.shape[0], table.dtype)
-        ctx.args = (scale, padding_id, dropout_p, seed, offset)
-        ctx.save_for_backward(ids, draw)
-        return _ext.embedding(table, ids, scale, padding_id, dtype, dropout_p, seed, offset, draw)
+        ctx.how = how
+        ctx.save_for_backward(ids, how[-1])
+        return _ext.embedding(table, ids, dtype, *how)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        ids, draw = ctx.saved_tensors
+        if grad.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("the gradient of embedding() cannot be differentiated again")
+        ids, _ = ctx.saved_tensors  # raises if the ids or the draw have changed since
         rows, dtype = ctx.table
         grad = grad.contiguous()
         target = ctx.leaf.grad if ctx.leaf is not None else None
-        with torch.cuda.nvtx.range("embedding_backward"):
-            if (target is not None and grad.dtype == torch.float32 and target.dtype == torch.float32
-                    and target.is_contiguous() and target.shape == (rows, grad.shape[-1])
-                    and target.device == grad.device):
-                _ext.embedding_backward_into(target, grad, ids, *ctx.args, draw)
-                return (None,) * 9
-            grad_table = _ext.embedding_backward(grad, ids, rows, dtype, *ctx.args, draw)
-        return (grad_table,) + (None,) * 8
+        if (target is not None and grad.dtype == torch.float32 and target.dtype == torch.float32
+                and target.is_contiguous() and target.shape == (rows, grad.shape[-1])
+                and target.device == grad.device):
+            _ext.embedding_backward_into(target, grad, ids, *ctx.how)
+            return None, None, None, None
+        return _ext.embedding_backward(grad, ids, rows, dtype, *ctx.how), None, None, None
 
 
 def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, padding_id: int | None = None,
@@ -64,5 +63,5 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, pad
     table = table.contiguous()
     ids = ids.contiguous()
     if table.requires_grad and torch.is_grad_enabled():
-        return Embedding.apply(table, ids, scale, padding_id, dtype, dropout_p, seed, offset, draw)
-    return _ext.embedding(table, ids, scale, padding_id, dtype, dropout_p, seed, offset, draw)
+        return Embedding.apply(table, ids, dtype, (scale, padding_id, dropout_p, seed, offset, draw))
+    return _ext.embedding(table, ids, dtype, scale, padding_id, dropout_p, seed, offset, draw)

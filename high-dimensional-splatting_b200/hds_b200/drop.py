@@ -11,16 +11,18 @@ class Dropout(torch.autograd.Function):
     """y = dropout(x); the backward is the same kernel on dL/dy under the same draw."""
 
     @staticmethod
-    def forward(ctx, x, p, seed, offset, rows, draw):
-        ctx.args = (p, seed, offset, rows)
-        ctx.save_for_backward(draw)
-        return _ext.dropout(x, p, seed, offset, rows, draw)
+    def forward(ctx, x, how):
+        """how: dropout()'s (p, seed, offset, rows, draw)."""
+        ctx.how = how
+        if how[-1] is not None:
+            ctx.save_for_backward(how[-1])
+        return _ext.dropout(x, *how)
 
     @staticmethod
     def backward(ctx, grad):
-        (draw,) = ctx.saved_tensors
-        p, seed, offset, rows = ctx.args
-        return dropout(grad, p, seed=seed, offset=offset, rows=rows, draw=draw), None, None, None, None, None
+        ctx.saved_tensors  # raises if the draw has changed since
+        p, seed, offset, rows, draw = ctx.how
+        return dropout(grad, p, seed=seed, offset=offset, rows=rows, draw=draw), None
 
 
 def dropout(x: torch.Tensor, p: float, *, seed: int = 0, offset: int = 0, rows: bool = False,
@@ -37,5 +39,5 @@ def dropout(x: torch.Tensor, p: float, *, seed: int = 0, offset: int = 0, rows: 
         return x
     x = x.contiguous()
     if x.requires_grad and torch.is_grad_enabled():
-        return Dropout.apply(x, p, seed, offset, rows, draw)
+        return Dropout.apply(x, (p, seed, offset, rows, draw))
     return _ext.dropout(x, p, seed, offset, rows, draw)

@@ -463,23 +463,25 @@ _DROP_ONE = 65536
 def drop_threshold(p: float) -> int:
     """The 16-bit threshold of a dropout probability: an element is dropped with probability
     round(65536 p) / 65536."""
-    p = float(p)
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout probability must be in [0, 1], got {p}")
-    return round(p * _DROP_ONE)
+    return round(float(p) * _DROP_ONE)
+
+
+_LOW64 = 0xFFFFFFFFFFFFFFFF
 
 
 def _draw(seed, offset, draw, device):
     """(seed, offset, draw pointer): the two numbers modulo 2^64, or the address of an int64 [2] tensor
     that holds them."""
     if draw is None:
-        return int(seed) & 0xFFFFFFFFFFFFFFFF, int(offset) & 0xFFFFFFFFFFFFFFFF, None
+        return int(seed) & _LOW64, int(offset) & _LOW64, None
     if draw.dtype != torch.int64 or draw.shape != (2,) or not draw.is_contiguous() or draw.device != device:
         raise RuntimeError("draw must be a contiguous int64 tensor [2] (seed, offset) on the input's device")
     return 0, 0, draw.data_ptr()
 
 
-def _check_table_ids(table_dtype, value_dtype, ids, device, padding_id):
+def _check_lookup(table_dtype, value_dtype, ids, device, padding_id):
     if table_dtype not in _FLOATS or (value_dtype is not table_dtype and value_dtype is not _F32):
         raise RuntimeError("the table must be float32, bfloat16 or float16, and its values of that type or float32")
     if ids.dtype not in _IDS:
@@ -492,7 +494,7 @@ def _check_table_ids(table_dtype, value_dtype, ids, device, padding_id):
         raise ValueError(f"padding_id {padding_id} does not fit 64 bits")
 
 
-def embedding(table, ids, scale: float = 1.0, padding_id: int | None = None, dtype=None, dropout_p: float = 0.0,
+def embedding(table, ids, dtype=None, scale: float = 1.0, padding_id: int | None = None, dropout_p: float = 0.0,
               seed: int = 0, offset: int = 0, draw=None):
     """scale * table[ids], with dropout of its elements in the same pass.  table [V, C] float32, bfloat16
     or float16; ids any shape, int32 or int64.  Returns [*ids.shape, C] of `dtype` (the table's type, the
@@ -507,7 +509,7 @@ def embedding(table, ids, scale: float = 1.0, padding_id: int | None = None, dty
         raise RuntimeError("table must be [V, C]")
     dtype = dtype or table.dtype
     dev = table.device
-    _check_table_ids(table.dtype, dtype, ids, dev, padding_id)
+    _check_lookup(table.dtype, dtype, ids, dev, padding_id)
     threshold = drop_threshold(dropout_p)
     seed, offset, draw_ptr = _draw(seed, offset, draw, dev)
     v, c = table.shape
@@ -525,16 +527,17 @@ def _embedding_backward(grad, ids, grad_table, accumulate, scale, padding_id, dr
     v, c = grad_table.shape
     if grad.device != dev or grad.shape != (*ids.shape, c):
         raise RuntimeError(f"grad must be {(*ids.shape, c)} on the table's device")
-    _check_table_ids(grad_table.dtype, grad.dtype, ids, dev, padding_id)
+    _check_lookup(grad_table.dtype, grad.dtype, ids, dev, padding_id)
     threshold = drop_threshold(dropout_p)
     seed, offset, draw_ptr = _draw(seed, offset, draw, dev)
     n = ids.numel()
-    scratch = torch.empty(lib.hds_embedding_backward_scratch_bytes(n, v, c), dtype=torch.uint8, device=dev)
+    need = lib.hds_embedding_backward_scratch_bytes(n, v, c)
+    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     with on_device(dev):
         check(lib.hds_embedding_backward(n, v, c, _TYPES[grad.dtype], grad.data_ptr(), _TYPES[ids.dtype],
                                          ids.data_ptr(), padding_id is not None, padding_id or 0, scale, threshold,
                                          seed, offset, draw_ptr, _TYPES[grad_table.dtype], grad_table.data_ptr(),
-                                         accumulate, scratch.data_ptr(), scratch.numel(), stream_of(dev)))
+                                         accumulate, ptr(scratch), need, stream_of(dev)))
 
 
 def embedding_backward(grad, ids, rows: int, dtype=None, scale: float = 1.0, padding_id: int | None = None,

@@ -108,7 +108,10 @@ class _LazyLib:
             raise AttributeError(name)
         if self._cdll is None:
             self._cdll = _load()
-        return getattr(self._cdll, name)
+        fn = getattr(self._cdll, name)
+        if name in SIGNATURES:
+            self.__dict__[name] = fn  # found without this detour from now on
+        return fn
 
 
 lib = _LazyLib()
@@ -126,17 +129,24 @@ def ptr(t) -> int | None:
 
 
 def stream_of(device) -> int:
+    """The current stream (a cudaStream_t) of a CUDA device (None: of the current one)."""
     import torch
 
+    if isinstance(device, torch.device) and device.type == "cuda" and device.index is not None:
+        # The raw handle: building torch.cuda.current_stream()'s object takes 2.4 us, this call 0.1.
+        return torch._C._cuda_getCurrentRawStream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_NO_CONTEXT = contextlib.nullcontext()
 
 
 def on_device(device):
     """Context in which `device` is the current CUDA device (the C ABI launches on the current one)."""
     import torch
 
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if device.index == torch._C._cuda_getDevice():
+        return _NO_CONTEXT
     return torch.cuda.device(device)
 
 

@@ -327,7 +327,8 @@ int hds_densify_apply(int n_old, int n_new, int segments, const int* widths, int
  * hds_embedding_backward: grad_table[v] = scale * sum of grad[i] over the i with ids[i] = v, in fp32 and
  * in an order that depends on the arguments alone: the same call gives the same bits.  accumulate != 0
  * (fp32 tables) adds it to what grad_table holds and leaves the rows of absent ids untouched; 0 writes
- * every row.  scratch: hds_embedding_backward_scratch_bytes(n, vocab, channels) bytes, 256-byte aligned.
+ * every row.  scratch: hds_embedding_backward_scratch_bytes(n, vocab, channels) bytes, 256-byte aligned
+ * (0 bytes, NULL, for few rows).
  *
  * hds_dropout: y = dropout(x), x and y [rows, channels] of one type; y may be x.  whole_rows drops whole
  * rows (e above is the row).  The gradient is the same call on dL/dy with the same draw.

@@ -15,9 +15,10 @@ namespace {
 // whatever V is, and the lane that holds an element fetches its group's decisions with a shuffle; with
 // 8-element vectors that is the lane itself.
 //
-// Whole rows: lane j draws for the rows 8 (r0 / 8 + j) .. + 7 around the tile's first row r0; a tile of rows
-// at least two wide spans at most 18 such groups.  Of rows at least V wide a vector meets two at most.
-// A vector all of whose rows are dropped is not read.
+// Whole rows: lane j draws for the rows 8 (r0 / 8 + j) .. + 7 from the tile's first row r0 on.  Of rows at
+// least 8 wide a warp's four tiles meet 130 at most, 18 such groups, so one generator call serves them all;
+// narrower rows take one for each tile.  Of rows at least V wide a vector meets two at most.  A vector
+// all of whose rows are dropped is not read.
 constexpr int DROPOUT_THREADS = 256;
 constexpr int TILE_ELEMENTS = 256;  // per warp
 constexpr int TILES = 4;            // tiles in flight per warp
@@ -95,11 +96,15 @@ __global__ void __launch_bounds__(DROPOUT_THREADS) dropout_rows_kernel(int64_t n
     };
     Vec<T, V> v[TILES][STEPS];
     uint32_t keep[TILES][STEPS];
+    uint32_t bits = 0;
+    int first = 0;  // of row0 among the decisions in bits
 #pragma unroll
     for (int t = 0; t < TILES; t++) {
-        const int64_t group0 = (row0 + rows_on(t * TILE_ELEMENTS)) >> 3;
-        const uint32_t bits = philox4x32_10((uint64_t)(group0 + lane), draw).bits(last);
-        const int first = (int)(row0 - 8 * group0);  // of row0 among the tile's decisions
+        if (t == 0 || row_width < 8) {
+            const int64_t group0 = (row0 + rows_on(t * TILE_ELEMENTS)) >> 3;
+            bits = philox4x32_10((uint32_t)(group0 + lane), (uint32_t)((uint64_t)(group0 + lane) >> 32), draw).bits(last);
+            first = (int)(row0 - 8 * group0);
+        }
         const auto row_kept = [&](uint32_t on) -> uint32_t {  // the row `on` rows from row0
             const int bit = first + (int)on;
             return (__shfl_sync(FULL_MASK, bits, bit >> 3) >> (bit & 7)) & 1u;
@@ -114,9 +119,9 @@ __global__ void __launch_bounds__(DROPOUT_THREADS) dropout_rows_kernel(int64_t n
             } else {
                 const uint32_t on = rows_on(at), on_end = rows_on(at + V - 1);
                 const uint32_t a = row_kept(on), b = row_kept(on_end);
-                // Elements of the vector in its first row.
-                const int64_t left = (int64_t)(on + 1) * row_width - place - at;
-                const uint32_t low = left >= V ? (1u << V) - 1u : (1u << (int)left) - 1u;
+                // The elements of the vector in its first row: all, or as many as lie before the next one.
+                uint32_t low = (1u << V) - 1u;
+                if (on_end != on) low = (1u << (int)((int64_t)on_end * row_width - place - at)) - 1u;
                 mine = (a ? low : 0u) | (b ? ((1u << V) - 1u) & ~low : 0u);
             }
             keep[t][k] = mine;

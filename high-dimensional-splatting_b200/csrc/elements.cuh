@@ -43,6 +43,7 @@ struct Vec {
             return to_float(*reinterpret_cast<const T*>(&h));
         }
     }
+    // In the order of k: the lower half of a word clears the upper.
     __device__ __forceinline__ void set(int k, float x) {
         if constexpr (sizeof(T) == 4) {
             w[k] = __float_as_uint(x);
@@ -51,6 +52,12 @@ struct Vec {
             const uint32_t h = *reinterpret_cast<const uint16_t*>(&v);
             w[k / 2] = k % 2 == 0 ? h : (w[k / 2] | (h << 16));
         }
+    }
+    __device__ __forceinline__ void clear(int k) {
+        if constexpr (sizeof(T) == 4)
+            w[k] = 0;
+        else
+            w[k / 2] &= k % 2 == 0 ? 0xffff0000u : 0xffffu;
     }
 };
 

@@ -25,122 +25,164 @@ namespace {
 
 inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
-struct Padding {
-    int present;
-    int64_t id;
-};
-
-// The table row of an id, or -1 for a row of zeros (padding, or outside the table: recorded).
-__device__ __forceinline__ int64_t table_row(int64_t v, int64_t vocab, const Padding& padding) {
-    if (padding.present && v == padding.id) return -1;
-    if (v < 0 || v >= vocab) {
-        atomicExch(&g_embedding_status, HDS_ERR_INVALID);
-        return -1;
-    }
-    return v;
-}
-
 constexpr int THREADS = 256;
 constexpr size_t DEFAULT_SHARED_BYTES = 48 << 10;  // a block may have more on request
+
+// The ids, and which table row each stands for.
+struct Ids {
+    const void* p;
+    int wide;        // int64 (else int32)
+    uint32_t vocab;
+    int padding_row;  // the padding id if it lies in the table, else -1
+    int has_padding;
+    int64_t padding_id;
+
+    // The table rows of the ids first, first + step, ... below n: -1 for a row of zeros (padding, or outside
+    // the table, which is recorded; and beyond n).  All are loaded before the first is looked at.
+    template <int COUNT>
+    __device__ __forceinline__ void rows(int first, int step, int n, int (&row)[COUNT]) const {
+        const int left = n - first;
+        if (wide)
+            classify<long long, unsigned long long, COUNT>(first, step, left, row);
+        else
+            classify<int, unsigned, COUNT>(first, step, left, row);
+    }
+
+private:
+    template <typename I, typename U, int COUNT>
+    __device__ __forceinline__ void classify(int first, int step, int left, int (&row)[COUNT]) const {
+        const I* from = static_cast<const I*>(p) + first;
+        I id[COUNT];
+#pragma unroll
+        for (int r = 0; r < COUNT; r++) id[r] = r * step < left ? __ldg(from + r * step) : (I)0;
+        bool outside = false;
+#pragma unroll
+        for (int r = 0; r < COUNT; r++) {
+            const bool inside = (U)id[r] < (U)vocab;  // negative ids are large ones
+            outside |= !inside;
+            row[r] = inside && (int)id[r] != padding_row && r * step < left ? (int)id[r] : -1;
+        }
+        if (outside) {
+#pragma unroll
+            for (int r = 0; r < COUNT; r++)
+                if (r * step < left && (U)id[r] >= (U)vocab && !(has_padding && (int64_t)id[r] == padding_id))
+                    atomicExch(&g_embedding_status, HDS_ERR_INVALID);
+        }
+    }
+};
+
+Ids make_ids(const void* p, int type, int64_t vocab, int has_padding, int64_t padding_id) {
+    const bool inside = has_padding && padding_id >= 0 && padding_id < vocab;
+    return Ids{p, type == HDS_TYPE_I64, (uint32_t)vocab, inside ? (int)padding_id : -1, has_padding, padding_id};
+}
 
 // ---------------------------------------------------------------------------------------------
 // lookup
 // ---------------------------------------------------------------------------------------------
-// A warp writes tiles of 256 consecutive output elements in vectors of V, the widest into which rows
-// split and to which both buffers are aligned.  All of a warp's ids are loaded first, then all of its
-// table vectors, then it stores: TILES x 8 elements in flight per lane cover the two dependent loads.
-// Dropout: lane j draws group j of the tile, the holder of an element fetches its group's decisions with
-// a shuffle (itself when V = 8).
-constexpr int TILE_ELEMENTS = 256;
-constexpr int TILES = 4;
-constexpr int LOOKUP_ELEMENTS = THREADS / 32 * TILE_ELEMENTS * TILES;  // per block
-
-struct Ids {
-    const void* p;
-    int wide;  // int64 (else int32)
-    __device__ __forceinline__ int64_t operator[](int64_t i) const {
-        return wide ? __ldg(static_cast<const long long*>(p) + i) : (int64_t)__ldg(static_cast<const int*>(p) + i);
-    }
-    // The ids first, first + step, ... below n (0 beyond), loaded together.
-    template <int COUNT>
-    __device__ __forceinline__ void load(int64_t first, int64_t step, int64_t n, int64_t (&id)[COUNT]) const {
-        if (wide) {
-#pragma unroll
-            for (int r = 0; r < COUNT; r++)
-                id[r] = first + r * step < n ? __ldg(static_cast<const long long*>(p) + first + r * step) : 0;
-        } else {
-#pragma unroll
-            for (int r = 0; r < COUNT; r++)
-                id[r] = first + r * step < n ? __ldg(static_cast<const int*>(p) + first + r * step) : 0;
-        }
-    }
-};
+// Rows in vectors of V elements, V the widest into which rows split and to which both buffers are aligned.
+// A thread keeps its column through a few rows: the ids are loaded first, then the table's vectors, then
+// the output is stored, and nothing but pointers moves from row to row.  The rows are as many as make 64
+// bytes of input or output per thread: with 32 and 128 bytes 1.18M x 512 fp32 from a table of 8192 rows
+// takes a tenth longer.
+template <typename T, typename O, int V>
+constexpr int WIDE_BYTES = V * (sizeof(O) > sizeof(T) ? (int)sizeof(O) : (int)sizeof(T));
+template <typename T, typename O, int V>
+constexpr int LOOKUP_PASSES = 64 / WIDE_BYTES<T, O, V> < 8 ? 64 / WIDE_BYTES<T, O, V> : 8;
 
 template <typename T, typename O, int V, bool DROP>
-__global__ void __launch_bounds__(THREADS) lookup_kernel(int64_t total, int64_t vocab, int channels, Divider rows_of,
-                                                         const T* __restrict__ table, Ids ids, Padding padding,
-                                                         float factor, uint32_t last, Draw draw,
-                                                         O* __restrict__ out) {
-    constexpr int STEPS = 8 / V;
+__global__ void __launch_bounds__(THREADS, DROP ? 8 : 1) lookup_rows_kernel(int n, int channels, int vectors, int rows_at_once,
+                                                              Divider vectors_of, const T* __restrict__ table, Ids ids,
+                                                              float factor, uint32_t last, Draw draw,
+                                                              O* __restrict__ out) {
+    static_assert(V == 8 || !DROP, "a thread draws for whole groups of eight");
+    constexpr int PASSES = LOOKUP_PASSES<T, O, V>;
     if (DROP) draw = resolve(draw);
-    const int lane = threadIdx.x & 31;
-    const int in_block = (threadIdx.x >> 5) * (TILE_ELEMENTS * TILES);
-    const int64_t warp_base = (int64_t)blockIdx.x * LOOKUP_ELEMENTS + in_block;
-    if (warp_base >= total) return;
-    // A block's groups share the upper counter word: its first is a multiple of their number.
-    const uint64_t group0 = (uint64_t)blockIdx.x * (LOOKUP_ELEMENTS / 8);
-    const int64_t row0 = warp_base / channels;
-    const uint32_t place = (uint32_t)(warp_base - row0 * channels);
-    int64_t id[TILES][STEPS];
+    const uint32_t r = vectors_of.quotient(threadIdx.x);
+    const int vector = (int)(blockIdx.y * THREADS + threadIdx.x - r * vectors_of.d);
+    if (r >= (uint32_t)rows_at_once || vector >= vectors) return;
+    const int row0 = blockIdx.x * (PASSES * rows_at_once) + r, left = n - row0;
+    int from[PASSES];
+    ids.rows<PASSES>(row0, rows_at_once, n, from);
+    const T* column = table + vector * V;
+    Vec<T, V> v[PASSES];
 #pragma unroll
-    for (int t = 0; t < TILES; t++)
+    for (int p = 0; p < PASSES; p++)
+        if (from[p] >= 0) v[p] = load_shared_data<T, V>(column + (int64_t)from[p] * channels);
+    O* to = out + (int64_t)row0 * channels + vector * V;
+    const uint32_t step = (uint32_t)rows_at_once * channels;
+    const uint32_t group = (uint32_t)row0 * vectors + vector;
 #pragma unroll
-        for (int k = 0; k < STEPS; k++) {
-            const uint32_t e = t * TILE_ELEMENTS + (k * 32 + lane) * V;
-            id[t][k] = warp_base + e < total ? ids[row0 + rows_of.quotient(place + e)] : 0;
-        }
-    int64_t at[TILES][STEPS];  // the vector's first element in the table, or -1
-#pragma unroll
-    for (int t = 0; t < TILES; t++)
-#pragma unroll
-        for (int k = 0; k < STEPS; k++) {
-            const uint32_t e = t * TILE_ELEMENTS + (k * 32 + lane) * V;
-            const int64_t row = warp_base + e < total ? table_row(id[t][k], vocab, padding) : -1;
-            const uint32_t q = rows_of.quotient(place + e);
-            at[t][k] = row < 0 ? -1 : row * channels + (place + e - q * channels);
-        }
-    Vec<T, V> v[TILES][STEPS];
-#pragma unroll
-    for (int t = 0; t < TILES; t++)
-#pragma unroll
-        for (int k = 0; k < STEPS; k++) {
-            v[t][k] = Vec<T, V>{};
-            if (at[t][k] >= 0) v[t][k] = load_shared_data<T, V>(table + at[t][k]);
-        }
-#pragma unroll
-    for (int t = 0; t < TILES; t++) {
+    for (int p = 0; p < PASSES; p++) {
         Numbers8 numbers{};
-        uint32_t bits = 0;
-        if (DROP) {
-            numbers = philox4x32_10((uint32_t)group0 + (in_block + t * TILE_ELEMENTS) / 8 + lane,
-                                    (uint32_t)(group0 >> 32), draw);
-            if (V < 8) bits = numbers.bits(last);
-        }
+        if (DROP) numbers = philox4x32_10(group + (uint32_t)(p * rows_at_once * vectors), 0, draw);
+        Vec<O, V> result;
 #pragma unroll
-        for (int k = 0; k < STEPS; k++) {
-            const int e = (k * 32 + lane) * V;
-            uint32_t mine = 0;
-            if (DROP && V < 8) mine = __shfl_sync(FULL_MASK, bits, e >> 3) >> (e & 7);
-            Vec<O, V> r;
+        for (int j = 0; j < V; j++) result.set(j, !DROP || numbers.kept(j, last) ? v[p].get(j) * factor : 0.0f);
+        if (from[p] < 0) result = Vec<O, V>{};
+        if (p * rows_at_once < left) store<O, V>(to + p * step, result);
+    }
+}
+
+// Rows that split into vectors of two at most, and dropout on rows that do not split into groups of eight.
+// Eight rows are whole groups, so a block takes `eights` times eight rows, group by group: one generator
+// call still serves eight elements, an id eight of its row's, and the output is one vector.  A group's elements
+// come from the table in vectors of V, from two rows at most (any number when rows are narrower than a
+// group).  (With a thread per element 1.18M x 75 fp32 took 174 us, GROUPS_US like this.)
+template <typename T, typename O, int V, bool DROP>
+__global__ void __launch_bounds__(THREADS) lookup_groups_kernel(int n, int channels, int eights, Divider rows_of,
+                                                                const T* __restrict__ table, Ids ids, float factor,
+                                                                uint32_t last, Draw draw, int whole,
+                                                                O* __restrict__ out) {
+    if (DROP) draw = resolve(draw);
+    const int groups = eights * channels;  // of the block
+    const int row0 = blockIdx.x * 8 * eights;
+    const uint64_t group0 = (uint64_t)blockIdx.x * groups;
+    const int64_t total = (int64_t)n * channels;
+    const auto row_of = [&](uint32_t e) -> int {
+        return rows_of.d != 0 ? (int)rows_of.quotient(e) : (int)(e / (uint32_t)channels);
+    };
+    for (int g = threadIdx.x; g < groups; g += THREADS) {
+        const int64_t first = (int64_t)(group0 + g) * 8;
+        if (first >= total) break;
+        Vec<T, V> v[8 / V];
+        uint32_t there = 0;  // bit j: element j comes from the table (its first row in the place of no row)
+        if (channels >= 8) {
+            const int q = row_of(8 * g), col = 8 * g - q * channels, left = channels - col;
+            int from[2];
+            ids.rows<2>(row0 + q, 1, n, from);
+            const uint32_t in_a = left >= 8 ? 0xffu : (1u << left) - 1u;
+            there = (from[0] >= 0 ? in_a : 0u) | (from[1] >= 0 ? 0xffu & ~in_a : 0u);
+            const T* a = table + (int64_t)max(from[0], 0) * channels + col;
+            const T* b = table + (int64_t)max(from[1], 0) * channels - left;
 #pragma unroll
-            for (int j = 0; j < V; j++) {
-                // A row of zeros stays one: its table vector was set to zero.
-                const bool kept = !DROP || (V == 8 ? numbers.kept(j, last) : ((mine >> j) & 1u) != 0);
-                r.set(j, kept ? v[t][k].get(j) * factor : 0.0f);
+            for (int k = 0; k < 8 / V; k++) v[k] = load_shared_data<T, V>((k * V < left ? a : b) + k * V);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8 / V; k++) {
+                const int q = row_of(8 * g + k * V);
+                int from[1];
+                ids.rows<1>(row0 + q, 1, n, from);
+                if (from[0] >= 0) there |= ((1u << V) - 1u) << (k * V);
+                v[k] = load_shared_data<T, V>(table + (int64_t)max(from[0], 0) * channels +
+                                              (8 * g + k * V - q * channels));
             }
-            const int64_t to = warp_base + t * TILE_ELEMENTS + e;
-            if (to < total) store<O, V>(out + to, r);
         }
+        Numbers8 numbers{};
+        if (DROP) numbers = philox4x32_10((uint32_t)group0 + g, 0, draw);
+        Vec<O, 8> r;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            r.set(j, !DROP || numbers.kept(j, last) ? v[j / V].get(j % V) * factor : 0.0f);
+        if (there != 0xffu) {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (!((there >> j) & 1u)) r.clear(j);
+        }
+        if (whole && first + 8 <= total)
+            store<O, 8>(out + first, r);
+        else
+            for (int j = 0; j < 8; j++)
+                if (first + j < total) out[first + j] = from_float<O>(r.get(j));
     }
 }
 
@@ -170,58 +212,50 @@ constexpr int MANY_ROUNDS = 16, SOME_ROUNDS = 4;
 constexpr int MAX_DIGIT_BITS = 11;
 constexpr int MAX_DIGITS = 1 << MAX_DIGIT_BITS;
 
-// The keys of a pass.  The first pass makes them from the ids; all of a thread's ids are loaded before the
-// first is looked at, since an id outside the table is recorded, a side effect that orders what follows.
-struct KeySource {
-    const uint32_t* keys;  // sorted so far, or NULL in the first pass:
-    const int32_t* rows;
+// A pass's elements, (key, row) pairs.  The first pass makes them from the ids; all of a thread's ids are
+// loaded before the first is looked at, since an id outside the table is recorded, a side effect that
+// orders what follows.
+struct PairSource {
+    const uint2* pairs;  // sorted so far, or NULL in the first pass:
     Ids ids;
-    Padding padding;
-    int64_t vocab;
 
-    // keys of the elements first, first + step, ... below n (0 beyond).
+    // The elements first, first + step, ... below n (key 0 beyond).
     template <int COUNT>
-    __device__ __forceinline__ void load(int64_t first, int step, int64_t n, uint32_t (&key)[COUNT]) const {
-        if (keys != nullptr) {
+    __device__ __forceinline__ void load(int first, int step, int n, uint2 (&pair)[COUNT]) const {
+        const int left = n - first;
+        if (pairs != nullptr) {
 #pragma unroll
-            for (int r = 0; r < COUNT; r++) key[r] = first + r * step < n ? __ldg(keys + first + r * step) : 0;
+            for (int r = 0; r < COUNT; r++)
+                pair[r] = r * step < left ? __ldg(pairs + first + r * step) : make_uint2(0, 0);
             return;
         }
-        int64_t id[COUNT];
-        ids.load<COUNT>(first, step, n, id);
+        int row[COUNT];
+        ids.rows<COUNT>(first, step, n, row);
 #pragma unroll
         for (int r = 0; r < COUNT; r++) {
-            const int64_t row = first + r * step < n ? table_row(id[r], vocab, padding) : 0;
-            key[r] = (uint32_t)(row < 0 ? vocab : row);
-        }
-    }
-    template <int COUNT>
-    __device__ __forceinline__ void load_rows(int64_t first, int step, int64_t n, int32_t (&row)[COUNT]) const {
-#pragma unroll
-        for (int r = 0; r < COUNT; r++) {
-            const int64_t i = first + r * step;
-            row[r] = rows == nullptr ? (int32_t)i : i < n ? __ldg(rows + i) : 0;
+            const uint32_t key = row[r] < 0 ? ids.vocab : (uint32_t)row[r];
+            pair[r] = make_uint2(r * step < left ? key : 0, (uint32_t)(first + r * step));
         }
     }
 };
 
 // counts[digit][tile] and totals[digit] (cleared by the caller; integer adds, so their order is no matter).
 template <int ROUNDS>
-__global__ void __launch_bounds__(SORT_THREADS) histogram_kernel(int64_t n, KeySource source, int shift, int bits,
+__global__ void __launch_bounds__(SORT_THREADS) histogram_kernel(int n, PairSource source, int shift, int bits,
                                                                  int tiles, uint32_t* __restrict__ counts,
                                                                  uint32_t* __restrict__ totals) {
     __shared__ uint32_t hist[MAX_DIGITS];
     const int digits = 1 << bits;
     for (int d = threadIdx.x; d < digits; d += SORT_THREADS) hist[d] = 0;
     __syncthreads();
-    const int64_t base = (int64_t)blockIdx.x * (SORT_THREADS * ROUNDS) + threadIdx.x;
+    const int base = blockIdx.x * (SORT_THREADS * ROUNDS) + threadIdx.x;
     const int lane = threadIdx.x & 31;
-    uint32_t key[ROUNDS];
-    source.load<ROUNDS>(base, SORT_THREADS, n, key);
+    uint2 pair[ROUNDS];
+    source.load<ROUNDS>(base, SORT_THREADS, n, pair);
 #pragma unroll
     for (int r = 0; r < ROUNDS; r++) {
         const bool valid = base + r * SORT_THREADS < n;
-        const uint32_t d = (key[r] >> shift) & (digits - 1);
+        const uint32_t d = (pair[r].x >> shift) & (digits - 1);
         // One shared atomic per distinct digit of the warp: popular codewords would serialise otherwise.
         const uint32_t peers = lanes_alike(d, bits, valid);
         if (valid && lane == __ffs(peers) - 1) atomicAdd(&hist[d], __popc(peers));
@@ -234,19 +268,18 @@ __global__ void __launch_bounds__(SORT_THREADS) histogram_kernel(int64_t n, KeyS
     }
 }
 
-// counts[digit][tile] -> the position of the tile's first key of that digit.  A warp per digit: its base
-// is the sum of the totals of all smaller digits, then a scan along the tiles.
+// A scatter block sums the counts of the tiles before its own itself where that takes few loads: a thread a
+// digit for 16 tiles at most, a warp a digit for 160 tiles and 256 digits at most.
+constexpr int FEW_TILES = 16, SOME_TILES = 160, SOME_DIGIT_BITS = 8;
+
+// counts[digit][tile] -> how many keys of that digit the tiles before have.  A warp per digit.
 constexpr int SCAN_WARPS = 8;
 
 __global__ void __launch_bounds__(32 * SCAN_WARPS) scan_kernel(int digits, int tiles,
-                                                               const uint32_t* __restrict__ totals,
                                                                uint32_t* __restrict__ counts) {
     const int lane = threadIdx.x & 31, digit = blockIdx.x * SCAN_WARPS + (threadIdx.x >> 5);
     if (digit >= digits) return;
     uint32_t base = 0;
-#pragma unroll 8
-    for (int d = lane; d < digit; d += 32) base += totals[d];
-    base = __reduce_add_sync(FULL_MASK, base);
     uint32_t* row = counts + (int64_t)digit * tiles;
     constexpr int AHEAD = 8;
     for (int t0 = lane; t0 < tiles + lane; t0 += 32 * AHEAD) {
@@ -267,33 +300,68 @@ __global__ void __launch_bounds__(32 * SCAN_WARPS) scan_kernel(int digits, int t
     }
 }
 
-// Each warp ranks its own consecutive keys into a count table of its own; a scan over the warps then
-// places the tables one after another.
-inline size_t scatter_shared_bytes(int digits) { return (size_t)digits * (sizeof(uint32_t) + 2 * SORT_WARPS); }
+// Each warp ranks its own consecutive keys into a count table of its own; a scan over the digits and the
+// warps places the tile's pairs in shared memory in sorted order, from where they go out in runs of equal
+// digits.  (Stored straight from the registers, each of a warp's pairs is a memory access of its own, and
+// the scatter of 1.18M pairs took 20 us instead of SCATTER_US.)
+inline size_t scatter_shared_bytes(int digits, int rounds) {
+    return (size_t)digits * (sizeof(uint32_t) + 2 * SORT_WARPS) + (size_t)rounds * SORT_THREADS * sizeof(uint2);
+}
 
 template <int ROUNDS>
-__global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(int64_t n, KeySource source, int shift, int bits,
-                                                               int tiles, const uint32_t* __restrict__ positions,
-                                                               uint32_t* __restrict__ keys_out,
-                                                               int32_t* __restrict__ rows_out) {
-    extern __shared__ uint32_t s_base[];                                  // [digits]
-    const int digits = 1 << bits;
-    uint16_t* s_warp = reinterpret_cast<uint16_t*>(s_base + digits);      // [warps][digits]
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t base = (int64_t)blockIdx.x * (SORT_THREADS * ROUNDS) + warp * (32 * ROUNDS) + lane;
+__global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(int n, PairSource source, int shift, int bits,
+                                                               int tiles, int scanned,
+                                                               const uint32_t* __restrict__ counts,
+                                                               const uint32_t* __restrict__ totals,
+                                                               uint2* __restrict__ out) {
+    constexpr int TILE = ROUNDS * SORT_THREADS;
+    constexpr int OWN = MAX_DIGITS / SORT_THREADS;  // digits per thread in the scan at most
+    extern __shared__ uint2 s_pair[];                                        // [TILE] in sorted order
+    __shared__ uint2 s_total[SORT_WARPS];
+    const int digits = 1 << bits, own = max(1, digits / SORT_THREADS);
+    uint32_t* s_move = reinterpret_cast<uint32_t*>(s_pair + TILE);           // [digits]: output - tile position
+    uint16_t* s_warp = reinterpret_cast<uint16_t*>(s_move + digits);         // [warps][digits]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tile = blockIdx.x * TILE;
+    const int base = tile + warp * (32 * ROUNDS) + lane;
     uint16_t* mine = s_warp + warp * digits;
-    uint32_t key[ROUNDS];
-    int32_t row[ROUNDS];
+    uint2 pair[ROUNDS];
     uint16_t rank[ROUNDS];
-    source.load<ROUNDS>(base, 32, n, key);
-    source.load_rows<ROUNDS>(base, 32, n, row);
-    for (int d = threadIdx.x; d < digits; d += SORT_THREADS) s_base[d] = positions[(int64_t)d * tiles + blockIdx.x];
-    for (int d = threadIdx.x; d < digits * SORT_WARPS / 2; d += SORT_THREADS) reinterpret_cast<uint32_t*>(s_warp)[d] = 0;
+    source.load<ROUNDS>(base, 32, n, pair);
+    // s_move for now: the digit's keys in the tiles before this one.
+    if (scanned) {
+        for (int d = tid; d < digits; d += SORT_THREADS) s_move[d] = counts[(int64_t)d * tiles + blockIdx.x];
+    } else if (tiles <= FEW_TILES) {
+        for (int d = tid; d < digits; d += SORT_THREADS) {
+            uint32_t before = 0;
+#pragma unroll
+            for (int t = 0; t < FEW_TILES; t++) before += t < (int)blockIdx.x ? counts[(int64_t)d * tiles + t] : 0;
+            s_move[d] = before;
+        }
+    } else {
+#pragma unroll 4
+        for (int d = warp; d < digits; d += SORT_WARPS) {
+            uint32_t before = 0;
+#pragma unroll
+            for (int t = lane; t < SOME_TILES; t += 32)
+                before += t < (int)blockIdx.x ? counts[(int64_t)d * tiles + t] : 0;
+            before = __reduce_add_sync(FULL_MASK, before);
+            if (lane == 0) s_move[d] = before;
+        }
+    }
+    uint32_t everywhere[OWN], sum_everywhere = 0;  // the digit's keys in all tiles
+#pragma unroll
+    for (int h = 0; h < OWN; h++) {
+        const int d = tid * own + h;
+        everywhere[h] = h < own && d < digits ? totals[d] : 0;
+        sum_everywhere += everywhere[h];
+    }
+    for (int i = tid; i < digits * SORT_WARPS / 2; i += SORT_THREADS) reinterpret_cast<uint32_t*>(s_warp)[i] = 0;
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < ROUNDS; r++) {
         const bool valid = base + 32 * r < n;
-        const uint32_t d = (key[r] >> shift) & (digits - 1);
+        const uint32_t d = (pair[r].x >> shift) & (digits - 1);
         const uint32_t peers = lanes_alike(d, bits, valid);
         const uint32_t before = mine[d];
         __syncwarp();
@@ -302,8 +370,38 @@ __global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(int64_t n, KeySou
         __syncwarp();
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < digits; d += SORT_THREADS) {
-        uint32_t run = 0;
+    // Where each digit, and in it each warp, starts in the tile.
+    uint32_t total[OWN], sum = 0;
+#pragma unroll
+    for (int h = 0; h < OWN; h++) {
+        const int d = tid * own + h;
+        total[h] = 0;
+        if (h < own && d < digits)
+#pragma unroll
+            for (int w = 0; w < SORT_WARPS; w++) total[h] += s_warp[w * digits + d];
+        sum += total[h];
+    }
+    uint32_t inclusive = sum, inclusive_everywhere = sum_everywhere;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(FULL_MASK, inclusive, o);
+        const uint32_t z = __shfl_up_sync(FULL_MASK, inclusive_everywhere, o);
+        if (lane >= o) inclusive += y;
+        if (lane >= o) inclusive_everywhere += z;
+    }
+    if (lane == 31) s_total[warp] = make_uint2(inclusive, inclusive_everywhere);
+    __syncthreads();
+    uint32_t run = inclusive - sum, start = inclusive_everywhere - sum_everywhere;
+    for (int w = 0; w < warp; w++) {
+        run += s_total[w].x;
+        start += s_total[w].y;
+    }
+#pragma unroll
+    for (int h = 0; h < OWN; h++) {
+        const int d = tid * own + h;
+        if (h >= own || d >= digits) break;
+        s_move[d] += start - run;
+        start += everywhere[h];
 #pragma unroll
         for (int w = 0; w < SORT_WARPS; w++) {
             const uint32_t c = s_warp[w * digits + d];
@@ -315,10 +413,17 @@ __global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(int64_t n, KeySou
 #pragma unroll
     for (int r = 0; r < ROUNDS; r++) {
         if (base + 32 * r >= n) break;
-        const uint32_t d = (key[r] >> shift) & (digits - 1);
-        const uint32_t pos = s_base[d] + mine[d] + rank[r];
-        keys_out[pos] = key[r];
-        rows_out[pos] = row[r];
+        const uint32_t d = (pair[r].x >> shift) & (digits - 1);
+        s_pair[mine[d] + rank[r]] = pair[r];
+    }
+    __syncthreads();
+    const int here = min(TILE, n - tile);
+#pragma unroll
+    for (int r = 0; r < ROUNDS; r++) {
+        const int i = tid + r * SORT_THREADS;
+        if (i >= here) break;
+        const uint2 p = s_pair[i];
+        out[s_move[(p.x >> shift) & (digits - 1)] + i] = p;
     }
 }
 
@@ -342,11 +447,12 @@ __device__ __forceinline__ void store_sum(T* p, const float* sum, float factor) 
     store<T, V>(p, r);
 }
 
+// Three blocks an SM (85 registers a thread) take 1.18M x 512 with dropout from 598 to 532 us; narrow vectors
+// would spill.
 template <typename G, typename T, int V, bool DROP, bool ACCUMULATE>
-__global__ void __launch_bounds__(THREADS) chunk_sum_kernel(int64_t n, uint32_t vocab, int channels, int slab,
+__global__ void __launch_bounds__(THREADS, V == COLUMNS ? 3 : 0) chunk_sum_kernel(int64_t n, uint32_t vocab, int channels, int slab,
                                                             int lanes_log2, int chunk,
-                                                            const uint32_t* __restrict__ keys,
-                                                            const int32_t* __restrict__ rows,
+                                                            int slabs, const uint2* __restrict__ pairs,
                                                             const G* __restrict__ grad, float factor,
                                                             uint32_t last, Draw draw, T* __restrict__ table,
                                                             float* __restrict__ heads, float* __restrict__ tails,
@@ -354,12 +460,16 @@ __global__ void __launch_bounds__(THREADS) chunk_sum_kernel(int64_t n, uint32_t 
     constexpr int STEPS = COLUMNS / V;
     if (DROP) draw = resolve(draw);
     const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1);
-    const int64_t id = ((int64_t)blockIdx.x * THREADS + threadIdx.x) >> lanes_log2;  // of the chunk
+    // The slabs of the same chunks are neighbouring blocks, so that they read the rows' halves together.
+    const int slab_id = blockIdx.x % slabs;
+    const int64_t id = ((int64_t)(blockIdx.x / slabs) * THREADS + threadIdx.x) >> lanes_log2;  // of the chunk
     const int64_t start = id * chunk;
-    const int c0 = blockIdx.y * slab, width = min(slab, channels - c0);
-    const auto column = [&](int k) { return (k * lanes + lane) * V; };  // within the slab
-    uint32_t current = start < n ? keys[start] : vocab;
-    bool began_earlier = start < n && start > 0 && keys[start - 1] == current;
+    const int c0 = slab_id * slab, width = min(slab, channels - c0);
+    // A lane's vector k, within the slab: interleaved between the lanes, so that narrow vectors coalesce; with
+    // dropout the lane's columns are consecutive, since then eight decisions are two neighbouring groups'.
+    const auto column = [&](int k) { return DROP ? lane * COLUMNS + k * V : (k * lanes + lane) * V; };
+    uint32_t current = start < n ? pairs[start].x : vocab;
+    bool began_earlier = start < n && start > 0 && pairs[start - 1].x == current;
     float sum[COLUMNS];
 #pragma unroll
     for (int j = 0; j < COLUMNS; j++) sum[j] = 0.0f;
@@ -381,49 +491,44 @@ __global__ void __launch_bounds__(THREADS) chunk_sum_kernel(int64_t n, uint32_t 
     };
 
     for (int p = 0; p < chunk; p += ROWS_AHEAD) {
-        // Chunks start at multiples of 8, so the four keys and rows are two 16-byte loads (the buffers are
-        // padded beyond n).
+        // Chunks start at multiples of 8, so the four pairs are two 16-byte loads (the buffers are padded
+        // beyond n).
         const int64_t pos = start + p;
-        uint4 key4 = make_uint4(vocab, vocab, vocab, vocab);
-        int4 row4 = make_int4(0, 0, 0, 0);
+        uint4 two[2] = {make_uint4(vocab, 0, vocab, 0), make_uint4(vocab, 0, vocab, 0)};
         if (pos < n) {
-            key4 = __ldg(reinterpret_cast<const uint4*>(keys + pos));
-            row4 = __ldg(reinterpret_cast<const int4*>(rows + pos));
+            two[0] = __ldg(reinterpret_cast<const uint4*>(pairs + pos));
+            two[1] = __ldg(reinterpret_cast<const uint4*>(pairs + pos) + 1);
         }
-        const uint32_t key[ROWS_AHEAD] = {key4.x, pos + 1 < n ? key4.y : vocab, pos + 2 < n ? key4.z : vocab,
-                                          pos + 3 < n ? key4.w : vocab};
-        const int32_t row[ROWS_AHEAD] = {row4.x, row4.y, row4.z, row4.w};
+        const uint32_t key[ROWS_AHEAD] = {two[0].x, pos + 1 < n ? two[0].z : vocab, pos + 2 < n ? two[1].x : vocab,
+                                          pos + 3 < n ? two[1].z : vocab};
+        const uint32_t row[ROWS_AHEAD] = {two[0].y, two[0].w, two[1].y, two[1].w};
         Vec<G, V> g[ROWS_AHEAD][STEPS];
 #pragma unroll
         for (int u = 0; u < ROWS_AHEAD; u++)
 #pragma unroll
             for (int k = 0; k < STEPS; k++)
                 if (key[u] != vocab && column(k) < width)
-                    g[u][k] = load_once<G, V>(grad + (int64_t)row[u] * channels + c0 + column(k));
-        Numbers8 numbers[ROWS_AHEAD];
-        uint32_t keep[ROWS_AHEAD][STEPS];
-        if (DROP) {
-#pragma unroll
-            for (int u = 0; u < ROWS_AHEAD; u++) {
-                const int64_t e = (int64_t)(key[u] != vocab ? row[u] : 0) * channels + c0;
-                numbers[u] = philox4x32_10((uint64_t)(e >> 3) + lane, draw);
-                if (V < COLUMNS) {
-                    const uint32_t bits = numbers[u].bits(last);
-                    // The row may start inside a group: its last columns then belong to one group more.
-                    const int into = (int)(e & 7);
-                    const uint32_t more =
-                        into + width > 8 * lanes ? philox4x32_10((uint64_t)(e >> 3) + lanes, draw).bits(last) : 0;
-#pragma unroll
-                    for (int k = 0; k < STEPS; k++) {
-                        const int b = into + column(k);
-                        const uint32_t theirs = __shfl_sync(FULL_MASK, bits, b >> 3, lanes);
-                        keep[u][k] = ((b >> 3) < lanes ? theirs : more) >> (b & 7);
-                    }
-                }
-            }
-        }
+                    g[u][k] = DROP && V < COLUMNS
+                                  ? load_shared_data<G, V>(grad + (int64_t)row[u] * channels + c0 + column(k))
+                                  : load_once<G, V>(grad + (int64_t)row[u] * channels + c0 + column(k));
 #pragma unroll
         for (int u = 0; u < ROWS_AHEAD; u++) {
+            Numbers8 numbers{};
+            uint32_t keep = 0;
+            if (DROP) {
+                const int64_t e = (int64_t)(key[u] != vocab ? row[u] : 0) * channels + c0;
+                numbers = philox4x32_10((uint32_t)(e >> 3) + lane, 0, draw);
+                if (V < COLUMNS) {
+                    // A row may start inside a group: a lane's columns are then the end of one group and the
+                    // beginning of the next lane's.
+                    const int into = (int)(e & 7);
+                    const uint32_t bits = numbers.bits(last);
+                    uint32_t next = __shfl_down_sync(FULL_MASK, bits, 1, lanes);
+                    if (into != 0 && lane == lanes - 1 && lane * COLUMNS + COLUMNS - into < width)
+                        next = philox4x32_10((uint32_t)(e >> 3) + lanes, 0, draw).bits(last);
+                    keep = (bits | next << 8) >> into;
+                }
+            }
             if (key[u] != current) {
                 if (current != vocab) finish();
                 current = key[u];
@@ -436,13 +541,13 @@ __global__ void __launch_bounds__(THREADS) chunk_sum_kernel(int64_t n, uint32_t 
             for (int k = 0; k < STEPS; k++)
 #pragma unroll
                 for (int j = 0; j < V; j++)
-                    if (!DROP || (V == COLUMNS ? numbers[u].kept(j, last) : ((keep[u][k] >> j) & 1u) != 0))
+                    if (!DROP || (V == COLUMNS ? numbers.kept(j, last) : ((keep >> (k * V + j)) & 1u) != 0))
                         sum[k * V + j] += g[u][k].get(j);
         }
     }
     if (current == vocab) return;
     const int64_t end = start + chunk;
-    if (end < n && keys[end] == current)
+    if (end < n && pairs[end].x == current)
         put(began_earlier ? heads : tails);
     else
         finish();
@@ -460,7 +565,7 @@ constexpr int HEADS_AHEAD = 8;  // probes, and heads loaded, at once
 
 template <typename T, int V, bool ACCUMULATE>
 __global__ void __launch_bounds__(THREADS) join_kernel(int64_t n, uint32_t vocab, int channels, int chunk,
-                                                       const uint32_t* __restrict__ keys,
+                                                       const uint2* __restrict__ pairs,
                                                        const float* __restrict__ heads,
                                                        const float* __restrict__ tails, int stride, float factor,
                                                        T* __restrict__ table) {
@@ -491,10 +596,10 @@ __global__ void __launch_bounds__(THREADS) join_kernel(int64_t n, uint32_t vocab
 
     const int64_t start = id * chunk, end = start + chunk;
     if (end < n) {
-        const uint32_t codeword = keys[end], at_end = keys[end - 1], at_start = keys[start];
-        const uint32_t before = start > 0 ? keys[start - 1] : vocab;
+        const uint32_t codeword = pairs[end].x, at_end = pairs[end - 1].x, at_start = pairs[start].x;
+        const uint32_t before = start > 0 ? pairs[start - 1].x : vocab;
         // The key with which the h-th chunk after the next one begins.
-        const auto key_after = [&](int h) { return id + 1 + h < chunks ? keys[(id + 1 + h) * chunk] : vocab; };
+        const auto key_after = [&](int h) { return id + 1 + h < chunks ? pairs[(id + 1 + h) * chunk].x : vocab; };
         uint32_t coarse[HEADS_AHEAD];
 #pragma unroll
         for (int h = 0; h < HEADS_AHEAD; h++) coarse[h] = key_after(HEADS_AHEAD * (h + 1));
@@ -529,13 +634,13 @@ __global__ void __launch_bounds__(THREADS) join_kernel(int64_t n, uint32_t vocab
     __syncthreads();
     for (int slot = 0; slot < s_long; slot++) {
         const int64_t from = s_id[slot];
-        const uint32_t codeword = keys[(from + 1) * chunk];
+        const uint32_t codeword = pairs[(from + 1) * chunk].x;
         // The last chunk that begins with the codeword lies in [last, beyond).
         int64_t last = from + 1, beyond = chunks;
         while (beyond - last > 1) {
             const int64_t step = (beyond - last + THREADS - 1) / THREADS;
             const int64_t probe = last + (threadIdx.x + 1) * step;
-            const int hits = __syncthreads_count(probe < beyond && keys[probe * chunk] == codeword);
+            const int hits = __syncthreads_count(probe < beyond && pairs[probe * chunk].x == codeword);
             last += hits * step;
             beyond = min(beyond, last + step);
         }
@@ -568,17 +673,19 @@ __global__ void __launch_bounds__(THREADS) join_kernel(int64_t n, uint32_t vocab
 // ---------------------------------------------------------------------------------------------
 // few rows: one launch
 // ---------------------------------------------------------------------------------------------
-// A block owns a range of codewords and 32 columns and does everything for them: it reads all ids, keeps
+// A block owns a range of codewords and a slab of columns and does everything for them: it reads all ids, keeps
 // the rows whose codeword is its own, groups them by codeword in shared memory (the scatter's ranking:
 // row order stays), adds each codeword's rows and writes every row of its range, zeros included.  Each
 // block reads all the ids, which is cheap while there are few; in return nothing waits for a second
-// launch.  A worker of 4 lanes (8 columns each) adds the rows of a codeword; one with many rows is added
-// by the whole block in 128 interleaved runs and a tree.
-constexpr int FEW_ROWS = 8192;
+// launch.  A worker of 1 to FEW_LANES lanes (8 columns each) adds the rows of a codeword; one with many rows
+// is added by the whole block, every worker a run of interleaved rows, and a tree.
 constexpr int FEW_THREADS = 512;
+constexpr int FEW_ROUNDS = 8;                        // ids per thread
+constexpr int FEW_ROWS = FEW_THREADS * FEW_ROUNDS;  // 4096
 constexpr int FEW_WARPS = FEW_THREADS / 32;
-constexpr int FEW_WORKERS = FEW_THREADS / JOIN_LANES;
+constexpr int FEW_LANES = 8;
 constexpr int FEW_RANGE = 2 * FEW_THREADS;  // codewords per block at most
+constexpr int FEW_VOCAB = 32768;            // beyond it, rows of zeros are better cleared by a memset
 constexpr int SHORT_ROWS = 32;
 
 inline size_t few_rows_shared_bytes(int64_t n, int range) {
@@ -586,21 +693,21 @@ inline size_t few_rows_shared_bytes(int64_t n, int range) {
 }
 
 template <typename G, typename T, int V, bool DROP, bool ACCUMULATE>
-__global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(int n, int64_t vocab, int channels, int range, Ids ids,
-                                                               Padding padding, const G* __restrict__ grad,
-                                                               float factor, uint32_t last, Draw draw,
+__global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(int n, int channels, int range, int lanes_log2, Ids ids,
+                                                               const G* __restrict__ grad, float factor,
+                                                               uint32_t last, Draw draw,
                                                                T* __restrict__ table) {
     constexpr int STEPS = COLUMNS / V;
     extern __shared__ uint32_t s_start[];                                    // [range + 1]
     uint16_t* s_count = reinterpret_cast<uint16_t*>(s_start + range + 1);    // [warps][range]
     uint16_t* s_rows = s_count + FEW_WARPS * range;                          // [n]
-    __shared__ float s_sum[FEW_WORKERS][JOIN_COLUMNS];
+    __shared__ float s_sum[FEW_THREADS * COLUMNS];                           // [workers][slab]
     __shared__ uint32_t s_warp[FEW_WARPS];
     __shared__ int s_long;
     __shared__ uint16_t s_long_codeword[FEW_ROWS / SHORT_ROWS];
     const int tid = threadIdx.x, warp = tid >> 5, lane32 = tid & 31;
-    const int64_t first = (int64_t)blockIdx.x * range;
-    const int here = (int)min((int64_t)range, vocab - first);
+    const int first = blockIdx.x * range;
+    const int here = min(range, (int)ids.vocab - first);
     const int bits = 32 - __clz(range - 1);  // of a codeword's number in the range
     if (DROP) draw = resolve(draw);
     for (int i = tid; i < FEW_WARPS * range; i += FEW_THREADS) s_count[i] = 0;
@@ -608,29 +715,21 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(int n, int64_t vo
     __syncthreads();
 
     // The block's rows by codeword: counts, positions, rows.
-    const int per_warp = (n + FEW_THREADS - 1) / FEW_THREADS * 32;
-    const int begin = warp * per_warp, end = min(n, begin + per_warp);
     uint16_t* mine = s_count + warp * range;
-    // The numbers in the range of the codewords of 4 x 32 rows (FEW_RANGE: not in it).
-    constexpr int BATCH = 4;
-    const auto local_codewords = [&](int i0, uint32_t (&d)[BATCH]) {
-        int64_t id[BATCH];
-        ids.load<BATCH>(i0 + lane32, 32, end, id);
+    const int base = warp * (32 * FEW_ROUNDS) + lane32;
+    int row[FEW_ROUNDS];
+    ids.rows<FEW_ROUNDS>(base, 32, n, row);
+    uint16_t rank[FEW_ROUNDS];  // among the warp's rows of the codeword
 #pragma unroll
-        for (int r = 0; r < BATCH; r++) {
-            const int64_t row = i0 + 32 * r + lane32 < end ? table_row(id[r], vocab, padding) : -1;
-            d[r] = row >= first && row < first + here ? (uint32_t)(row - first) : (uint32_t)FEW_RANGE;
-        }
-    };
-    for (int i0 = begin; i0 < end; i0 += 32 * BATCH) {
-        uint32_t d[BATCH];
-        local_codewords(i0, d);
-#pragma unroll
-        for (int r = 0; r < BATCH; r++) {
-            const uint32_t peers = lanes_alike(d[r], bits, d[r] < FEW_RANGE);
-            if (d[r] < FEW_RANGE && lane32 == __ffs(peers) - 1) mine[d[r]] = (uint16_t)(mine[d[r]] + __popc(peers));
-            __syncwarp();
-        }
+    for (int r = 0; r < FEW_ROUNDS; r++) {
+        row[r] = row[r] >= first && row[r] - first < here ? row[r] - first : -1;
+        const uint32_t d = (uint32_t)max(row[r], 0);
+        const uint32_t peers = lanes_alike(d, bits, row[r] >= 0);
+        const uint32_t before = mine[d];
+        __syncwarp();
+        rank[r] = (uint16_t)(before + __popc(peers & ((1u << lane32) - 1u)));
+        if (row[r] >= 0 && lane32 == __ffs(peers) - 1) mine[d] = (uint16_t)(before + __popc(peers));
+        __syncwarp();
     }
     __syncthreads();
     uint32_t total[2] = {0, 0};
@@ -661,27 +760,16 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(int n, int64_t vo
         if (d == here - 1) s_start[here] = run;
     }
     __syncthreads();
-    for (int i0 = begin; i0 < end; i0 += 32 * BATCH) {
-        uint32_t d[BATCH];
-        local_codewords(i0, d);
 #pragma unroll
-        for (int r = 0; r < BATCH; r++) {
-            const uint32_t peers = lanes_alike(d[r], bits, d[r] < FEW_RANGE);
-            const uint32_t at = d[r] < FEW_RANGE ? mine[d[r]] : 0;
-            __syncwarp();
-            if (d[r] < FEW_RANGE) {
-                s_rows[at + __popc(peers & ((1u << lane32) - 1u))] = (uint16_t)(i0 + 32 * r + lane32);
-                if (lane32 == __ffs(peers) - 1) mine[d[r]] = (uint16_t)(at + __popc(peers));
-            }
-            __syncwarp();
-        }
-    }
+    for (int r = 0; r < FEW_ROUNDS; r++)
+        if (row[r] >= 0) s_rows[mine[row[r]] + rank[r]] = (uint16_t)(base + 32 * r);
     __syncthreads();
 
-    const int worker = tid / JOIN_LANES, lane = tid % JOIN_LANES;
-    const unsigned worker_mask = 0xfu << (lane32 & ~(JOIN_LANES - 1));
-    const int c0 = blockIdx.y * JOIN_COLUMNS, width = min(JOIN_COLUMNS, channels - c0);
-    const auto column = [&](int k) { return (k * JOIN_LANES + lane) * V; };
+    const int lanes = 1 << lanes_log2, worker = tid >> lanes_log2, lane = tid & (lanes - 1);
+    const int workers = FEW_THREADS >> lanes_log2, slab = lanes * COLUMNS;
+    const unsigned worker_mask = (0xffffffffu >> (32 - lanes)) << (lane32 & ~(lanes - 1));
+    const int c0 = blockIdx.y * slab, width = min(slab, channels - c0);
+    const auto column = [&](int k) { return (k * lanes + lane) * V; };
     // sum += rows from, from + step, ... below to.
     const auto add_rows = [&](float* sum, uint32_t from, uint32_t to, uint32_t step) {
         for (uint32_t p = from; p < to; p += ROWS_AHEAD * step) {
@@ -697,18 +785,18 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(int n, int64_t vo
                     if (keep[u][k]) g[u][k] = load_once<G, V>(grad + e + column(k));
                 }
                 if (DROP) {
-                    const uint32_t bits = philox4x32_10((uint64_t)(e >> 3) + lane, draw).bits(last);
+                    const uint32_t bits = philox4x32_10((uint32_t)(e >> 3) + lane, 0, draw).bits(last);
                     const int into = (int)(e & 7);
-                    const uint32_t more = V < COLUMNS && into + width > JOIN_COLUMNS
-                                              ? philox4x32_10((uint64_t)(e >> 3) + JOIN_LANES, draw).bits(last)
+                    const uint32_t more = V < COLUMNS && into + width > slab
+                                              ? philox4x32_10((uint32_t)(e >> 3) + lanes, 0, draw).bits(last)
                                               : 0;
 #pragma unroll
                     for (int k = 0; k < STEPS; k++) {
                         const int b = into + column(k);
                         uint32_t theirs = bits;
                         if (V < COLUMNS) {
-                            theirs = __shfl_sync(worker_mask, bits, b >> 3, JOIN_LANES);
-                            theirs = ((b >> 3) < JOIN_LANES ? theirs : more) >> (b & 7);
+                            theirs = __shfl_sync(worker_mask, bits, b >> 3, lanes);
+                            theirs = ((b >> 3) < lanes ? theirs : more) >> (b & 7);
                         }
                         keep[u][k] &= theirs;
                     }
@@ -727,10 +815,10 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(int n, int64_t vo
 #pragma unroll
         for (int k = 0; k < STEPS; k++)
             if (column(k) < width)
-                store_sum<T, V, ACCUMULATE>(table + (first + codeword) * channels + c0 + column(k), sum + k * V,
+                store_sum<T, V, ACCUMULATE>(table + (int64_t)(first + codeword) * channels + c0 + column(k), sum + k * V,
                                             factor);
     };
-    for (int v = worker; v < here; v += FEW_WORKERS) {
+    for (int v = worker; v < here; v += workers) {
         const uint32_t from = s_start[v], to = s_start[v + 1];
         if (ACCUMULATE && from == to) continue;
         if (to - from > SHORT_ROWS) {
@@ -745,33 +833,25 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(int n, int64_t vo
     for (int slot = 0; slot < s_long; slot++) {
         const int v = s_long_codeword[slot];
         float sum[COLUMNS] = {};
-        add_rows(sum, s_start[v] + worker, s_start[v + 1], FEW_WORKERS);
+        add_rows(sum, s_start[v] + worker, s_start[v + 1], workers);
 #pragma unroll
-        for (int j = 0; j < COLUMNS; j++) s_sum[worker][lane * COLUMNS + j] = sum[j];
+        for (int k = 0; k < STEPS; k++)
+#pragma unroll
+            for (int j = 0; j < V; j++) s_sum[worker * slab + column(k) + j] = sum[k * V + j];
         __syncthreads();
-        for (int half = FEW_WORKERS / 2; half > 0; half /= 2) {
-            for (int i = tid; i < half * JOIN_COLUMNS; i += FEW_THREADS)
-                s_sum[i / JOIN_COLUMNS][i % JOIN_COLUMNS] += s_sum[i / JOIN_COLUMNS + half][i % JOIN_COLUMNS];
+        for (int half = workers / 2; half > 0; half /= 2) {
+            for (int i = tid; i < half * slab; i += FEW_THREADS) s_sum[i] += s_sum[i + half * slab];
             __syncthreads();
         }
-        if (worker == 0) write(v, s_sum[0] + lane * COLUMNS);
+        if (worker == 0) {
+#pragma unroll
+            for (int k = 0; k < STEPS; k++)
+#pragma unroll
+                for (int j = 0; j < V; j++) sum[k * V + j] = s_sum[column(k) + j];
+            write(v, sum);
+        }
         __syncthreads();
     }
-}
-
-// Codewords per block: enough blocks to fill the machine, at most FEW_RANGE codewords each.
-int few_rows_range(int64_t vocab, int channels) {
-    const int64_t slabs = (channels + JOIN_COLUMNS - 1) / JOIN_COLUMNS;
-    const int64_t blocks = std::max<int64_t>((vocab + FEW_RANGE - 1) / FEW_RANGE, std::min(vocab, 444 / slabs + 1));
-    return (int)((vocab + blocks - 1) / blocks);
-}
-
-// Few rows, and the blocks' reads of all ids together no more than 16M.
-bool few_rows(int64_t n, int64_t vocab, int channels) {
-    if (n > FEW_ROWS || vocab == 0 || channels == 0) return false;
-    const int64_t slabs = (channels + JOIN_COLUMNS - 1) / JOIN_COLUMNS;
-    const int range = few_rows_range(vocab, channels);
-    return (vocab + range - 1) / range * slabs * n <= (int64_t(1) << 24);
 }
 
 int ceil_log2(int64_t x) {
@@ -780,15 +860,34 @@ int ceil_log2(int64_t x) {
     return bits;
 }
 
+struct FewRowsPlan {
+    int lanes_log2, range;  // codewords per block: enough blocks to fill the machine, FEW_RANGE codewords at most
+    int64_t slabs, ranges;
+    bool fits;              // few rows, and blocks that all run in two or three waves
+    FewRowsPlan(int64_t n, int64_t vocab, int channels) {
+        lanes_log2 = ceil_log2(std::min(FEW_LANES, std::max(1, (channels + COLUMNS - 1) / COLUMNS)));
+        slabs = (channels + (COLUMNS << lanes_log2) - 1) / (COLUMNS << lanes_log2);
+        if (n == 0 || n > FEW_ROWS || vocab == 0 || channels == 0) {
+            fits = false;
+            return;
+        }
+        ranges = std::max<int64_t>((vocab + FEW_RANGE - 1) / FEW_RANGE, std::min(vocab, 444 / slabs + 1));
+        range = (int)((vocab + ranges - 1) / ranges);
+        ranges = (vocab + range - 1) / range;
+        fits = vocab <= FEW_VOCAB && ranges * slabs <= 2048;
+    }
+};
+
 // How the backward splits its work and lays out its scratch.
 struct BackwardPlan {
     int rounds;               // of the sort, per thread of a tile
     int64_t tiles;
     int passes, digit_bits;
+    int scan;                 // whether a kernel of its own sums the tiles' counts
     int chunk, stride;        // rows per chunk; floats per partial row
     int64_t chunks;
     int slab, lanes_log2;     // columns and lanes of a worker
-    size_t keys_a, keys_b, rows_a, rows_b, counts, totals, heads, tails, bytes;
+    size_t pairs_a, pairs_b, counts, totals, heads, tails, bytes;
 
     BackwardPlan(int64_t n, int64_t vocab, int channels) {
         const size_t nn = (size_t)std::max<int64_t>(n, 1);
@@ -797,6 +896,7 @@ struct BackwardPlan {
         const int bits = std::max(1, ceil_log2(vocab + 1));  // keys 0 .. vocab
         passes = (bits + MAX_DIGIT_BITS - 1) / MAX_DIGIT_BITS;
         digit_bits = (bits + passes - 1) / passes;
+        scan = !(tiles <= FEW_TILES || (tiles <= SOME_TILES && digit_bits <= SOME_DIGIT_BITS));
         // Long chunks write few partial sums (two rows of a chunk at most); but the chunks have to fill the
         // machine.  75,000 lanes with four rows of 32 bytes each in flight are about 10 MB, more than the
         // memory's latency times its rate.
@@ -808,11 +908,9 @@ struct BackwardPlan {
         const int slabs = std::max(1, (channels + 32 * COLUMNS - 1) / (32 * COLUMNS));
         slab = ((channels + slabs - 1) / slabs + COLUMNS - 1) / COLUMNS * COLUMNS;
         lanes_log2 = ceil_log2(std::max(slab / COLUMNS, 1));
-        keys_a = 0;
-        keys_b = keys_a + align256(nn * 4);
-        rows_a = keys_b + align256(nn * 4);
-        rows_b = rows_a + align256(nn * 4);
-        counts = rows_b + align256(nn * 4);
+        pairs_a = 0;
+        pairs_b = pairs_a + align256(nn * sizeof(uint2));
+        counts = pairs_b + align256(nn * sizeof(uint2));
         totals = counts + align256(((size_t)tiles << digit_bits) * 4);
         heads = totals + align256(((size_t)passes << digit_bits) * 4);
         tails = heads + align256((size_t)chunks * stride * 4);
@@ -824,7 +922,9 @@ struct BackwardPlan {
 int check_arguments(const char* what, int64_t n, int64_t vocab, int channels, int table_type, int value_type,
                     int ids_type, double scale, int drop_threshold) {
     HDS_REQUIRE(n >= 0 && vocab >= 0 && channels >= 0, HDS_ERR_INVALID, "%s: negative size", what);
-    HDS_REQUIRE(n < INT32_MAX && vocab < INT32_MAX && channels <= HDS_EMBEDDING_MAX_CHANNELS, HDS_ERR_TOO_LARGE,
+    // Row numbers are 32-bit, also of the last, partly empty, block.
+    constexpr int64_t most = INT32_MAX - (1 << 20);
+    HDS_REQUIRE(n <= most && vocab <= most && channels <= HDS_EMBEDDING_MAX_CHANNELS, HDS_ERR_TOO_LARGE,
                 "%s: n = %lld, vocab = %lld, channels = %d is too large", what, (long long)n, (long long)vocab,
                 channels);
     HDS_REQUIRE(known_type(table_type) && (value_type == table_type || value_type == HDS_TYPE_F32),
@@ -834,6 +934,9 @@ int check_arguments(const char* what, int64_t n, int64_t vocab, int channels, in
     HDS_REQUIRE(scale - scale == 0.0, HDS_ERR_INVALID, "%s: scale must be finite", what);
     HDS_REQUIRE(drop_threshold >= 0 && drop_threshold <= DROP_ONE, HDS_ERR_INVALID,
                 "%s: dropout threshold %d outside 0 to 65536", what, drop_threshold);
+    // The kernels keep the generator's upper group word out of the lanes: it is 0.
+    HDS_REQUIRE(drop_threshold == 0 || n * channels <= HDS_EMBEDDING_MAX_DROPOUT, HDS_ERR_TOO_LARGE,
+                "%s: dropout of %lld values (2^35 at most)", what, (long long)(n * channels));
     return HDS_OK;
 }
 
@@ -876,36 +979,60 @@ extern "C" int hds_embedding_forward(int64_t n, int64_t vocab, int channels, int
     HDS_REQUIRE(!misaligned(table, element_size(table_type)) && !misaligned(out, element_size(out_type)) &&
                     !misaligned(ids, ids_type == HDS_TYPE_I32 ? 4 : 8) && !misaligned(draw, 8),
                 HDS_ERR_INVALID, "embedding: misaligned buffer");
-    const Padding padding{has_padding, padding_id};
+    const Ids id = make_ids(ids, ids_type, vocab, has_padding, padding_id);
     const Draw d{seed, offset, draw};
     const float factor = keep_factor(scale, drop_threshold);
-    const int64_t total = n * channels;
-    const int64_t blocks = (total + LOOKUP_ELEMENTS - 1) / LOOKUP_ELEMENTS;
-    HDS_REQUIRE(blocks <= INT32_MAX, HDS_ERR_TOO_LARGE, "embedding: n = %lld, channels = %d is too large",
-                (long long)n, channels);
-    const Ids id{ids, ids_type == HDS_TYPE_I64};
-    const Divider rows_of = divider((uint32_t)channels);
+    const int v = widest_vector(channels, {{table, table_type}, {out, out_type}});
     return with_types(table_type, out_type, [&](auto t, auto o) -> int {
         using T = decltype(t);
         using O = decltype(o);
-        return with_vector(widest_vector(channels, {{table, table_type}, {out, out_type}}), [&](auto width) -> int {
-            constexpr int V = decltype(width)::value;
-            if (drop_threshold > 0)
-                lookup_kernel<T, O, V, true><<<(unsigned)blocks, THREADS, 0, stream>>>(
-                    total, vocab, channels, rows_of, static_cast<const T*>(table), id, padding, factor,
-                    below_last(drop_threshold), d, static_cast<O*>(out));
-            else
-                lookup_kernel<T, O, V, false><<<(unsigned)blocks, THREADS, 0, stream>>>(
-                    total, vocab, channels, rows_of, static_cast<const T*>(table), id, padding, factor, 0u, d,
-                    static_cast<O*>(out));
-            HDS_CHECK_LAUNCH("lookup_kernel");
+        const T* from = static_cast<const T*>(table);
+        O* to = static_cast<O*>(out);
+        // (A table without rows goes by rows: that kernel reads none of a row of zeros.)
+        if (v == 8 || (drop_threshold == 0 && v == 4) || vocab == 0) {
+            const int vectors = channels / (v == 2 ? 1 : v);
+            const int rows_at_once = std::max(1, THREADS / vectors);
+            const int threads = std::min(THREADS, (rows_at_once * vectors + 31) / 32 * 32);
+            // A row's threads: all of a block's when it has more vectors than a block has threads.
+            const Divider vectors_of = divider((uint32_t)std::min(vectors, THREADS));
+            const auto run = [&](auto* kernel, int passes) -> int {
+                const int64_t rows = (int64_t)passes * rows_at_once;  // of a block
+                const dim3 grid((unsigned)((n + rows - 1) / rows), (unsigned)((vectors + THREADS - 1) / THREADS));
+                kernel<<<grid, threads, 0, stream>>>((int)n, channels, vectors, rows_at_once, vectors_of, from, id,
+                                                     factor, below_last(drop_threshold), d, to);
+                HDS_CHECK_LAUNCH("lookup_rows_kernel");
+                return HDS_OK;
+            };
+            if (drop_threshold > 0 && v == 8) return run(lookup_rows_kernel<T, O, 8, true>, LOOKUP_PASSES<T, O, 8>);
+            if (v == 8) return run(lookup_rows_kernel<T, O, 8, false>, LOOKUP_PASSES<T, O, 8>);
+            if (v == 4) return run(lookup_rows_kernel<T, O, 4, false>, LOOKUP_PASSES<T, O, 4>);
+            return run(lookup_rows_kernel<T, O, 1, false>, LOOKUP_PASSES<T, O, 1>);
+        }
+        // Blocks of about 1024 groups.  Quotients of numbers below 8 eights channels (d = 0: too wide for them).
+        const int eights = std::max(1, 1024 / channels);
+        const Divider rows_of = channels <= 16384 ? divider((uint32_t)channels) : Divider{0, 0};
+        const unsigned blocks = (unsigned)((n + 8 * eights - 1) / (8 * eights));
+        const int whole = widest_vector(8, {{out, out_type}}) == 8;
+        const auto run = [&](auto* kernel) -> int {
+            kernel<<<blocks, THREADS, 0, stream>>>((int)n, channels, eights, rows_of, from, id, factor,
+                                                   below_last(drop_threshold), d, whole, to);
+            HDS_CHECK_LAUNCH("lookup_groups_kernel");
             return HDS_OK;
-        });
+        };
+        const int w = widest_vector(channels, {{table, table_type}});
+        if (drop_threshold > 0) {
+            if (w >= 4) return run(lookup_groups_kernel<T, O, 4, true>);
+            if (w == 2) return run(lookup_groups_kernel<T, O, 2, true>);
+            return run(lookup_groups_kernel<T, O, 1, true>);
+        }
+        if (w >= 4) return run(lookup_groups_kernel<T, O, 4, false>);
+        if (w == 2) return run(lookup_groups_kernel<T, O, 2, false>);
+        return run(lookup_groups_kernel<T, O, 1, false>);
     });
 }
 
 extern "C" size_t hds_embedding_backward_scratch_bytes(int64_t n, int64_t vocab, int channels) {
-    return few_rows(n, vocab, channels) ? 0 : BackwardPlan(n, vocab, channels).bytes;
+    return FewRowsPlan(n, vocab, channels).fits ? 0 : BackwardPlan(n, vocab, channels).bytes;
 }
 
 extern "C" int hds_embedding_backward(int64_t n, int64_t vocab, int channels, int grad_type, const void* grad,
@@ -923,19 +1050,19 @@ extern "C" int hds_embedding_backward(int64_t n, int64_t vocab, int channels, in
     HDS_REQUIRE(grad_table != nullptr && !misaligned(grad_table, element_size(table_type)), HDS_ERR_INVALID,
                 "embedding_backward: null or misaligned table gradient");
     const BackwardPlan plan(n, vocab, channels);
+    const FewRowsPlan few(n, vocab, channels);
     if (n > 0) {
         HDS_REQUIRE(grad != nullptr && ids != nullptr, HDS_ERR_INVALID, "embedding_backward: null pointer");
         HDS_REQUIRE(!misaligned(grad, element_size(grad_type)) && !misaligned(ids, ids_type == HDS_TYPE_I32 ? 4 : 8) &&
                         !misaligned(draw, 8),
                     HDS_ERR_INVALID, "embedding_backward: misaligned buffer");
-        HDS_REQUIRE(few_rows(n, vocab, channels) ||
+        HDS_REQUIRE(few.fits ||
                         (scratch != nullptr && scratch_bytes >= plan.bytes && !misaligned(scratch, 256)),
                     HDS_ERR_SCRATCH, "embedding_backward: scratch needs %zu bytes, 256-byte aligned", plan.bytes);
     }
     const Draw d{seed, offset, draw};
     const float factor = keep_factor(scale, drop_threshold);
-    const Ids id{ids, ids_type == HDS_TYPE_I64};
-    const Padding padding{has_padding, padding_id};
+    const Ids id = make_ids(ids, ids_type, vocab, has_padding, padding_id);
     const int v = widest_vector(channels, {{grad, grad_type}, {grad_table, table_type}});
     // Calls run(G{}, T{}, drop, add) with the types and the two switches.
     const auto with_variant = [&](auto&& run) -> int {
@@ -949,19 +1076,18 @@ extern "C" int hds_embedding_backward(int64_t n, int64_t vocab, int channels, in
                                       : run(g, t, std::false_type{}, std::false_type{});
         });
     };
-    if (n > 0 && few_rows(n, vocab, channels)) {
-        const int range = few_rows_range(vocab, channels);
-        const dim3 grid((unsigned)((vocab + range - 1) / range), (unsigned)((channels + JOIN_COLUMNS - 1) / JOIN_COLUMNS));
+    if (few.fits) {
+        const dim3 grid((unsigned)few.ranges, (unsigned)few.slabs);
         return with_variant([&](auto g, auto t, auto drop, auto add) -> int {
             using G = decltype(g);
             using T = decltype(t);
             const auto launch = [&](auto* kernel) -> int {
-                const size_t shared = few_rows_shared_bytes(n, range);
+                const size_t shared = few_rows_shared_bytes(n, few.range);
                 if (shared > DEFAULT_SHARED_BYTES / 2)  // with the kernel's own 17 KB
                     HDS_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                         (int)few_rows_shared_bytes(FEW_ROWS, FEW_RANGE)));
                 kernel<<<grid, FEW_THREADS, shared, stream>>>(
-                    (int)n, vocab, channels, range, id, padding, static_cast<const G*>(grad), factor,
+                    (int)n, channels, few.range, few.lanes_log2, id, static_cast<const G*>(grad), factor,
                     below_last(drop_threshold), d, static_cast<T*>(grad_table));
                 HDS_CHECK_LAUNCH("few_rows_kernel");
                 return HDS_OK;
@@ -977,49 +1103,46 @@ extern "C" int hds_embedding_backward(int64_t n, int64_t vocab, int channels, in
     if (n == 0) return HDS_OK;
 
     char* s = static_cast<char*>(scratch);
-    auto* keys = reinterpret_cast<uint32_t*>(s + plan.keys_a);
-    auto* keys_other = reinterpret_cast<uint32_t*>(s + plan.keys_b);
-    auto* rows = reinterpret_cast<int32_t*>(s + plan.rows_a);
-    auto* rows_other = reinterpret_cast<int32_t*>(s + plan.rows_b);
+    auto* pairs = reinterpret_cast<uint2*>(s + plan.pairs_a);
+    auto* pairs_other = reinterpret_cast<uint2*>(s + plan.pairs_b);
     auto* counts = reinterpret_cast<uint32_t*>(s + plan.counts);
     auto* totals = reinterpret_cast<uint32_t*>(s + plan.totals);
     auto* heads = reinterpret_cast<float*>(s + plan.heads);
     auto* tails = reinterpret_cast<float*>(s + plan.tails);
     const int digits = 1 << plan.digit_bits, tiles = (int)plan.tiles;
     HDS_CHECK_CUDA(cudaMemsetAsync(totals, 0, (size_t)plan.passes * digits * 4, stream));
-    KeySource source{nullptr, nullptr, id, padding, vocab};
+    PairSource source{nullptr, id};
     for (int pass = 0; pass < plan.passes; pass++) {
         const int shift = pass * plan.digit_bits;
         const auto run = [&](auto* histogram, auto* scatter) -> int {
-            const size_t shared = scatter_shared_bytes(digits);
+            const size_t shared = scatter_shared_bytes(digits, plan.rounds);
             if (shared > DEFAULT_SHARED_BYTES)
                 HDS_CHECK_CUDA(cudaFuncSetAttribute(scatter, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                    (int)scatter_shared_bytes(MAX_DIGITS)));
-            histogram<<<tiles, SORT_THREADS, 0, stream>>>(n, source, shift, plan.digit_bits, tiles, counts,
+                                                    (int)scatter_shared_bytes(MAX_DIGITS, plan.rounds)));
+            histogram<<<tiles, SORT_THREADS, 0, stream>>>((int)n, source, shift, plan.digit_bits, tiles, counts,
                                                           totals + pass * digits);
             HDS_CHECK_LAUNCH("histogram_kernel");
-            scan_kernel<<<(digits + SCAN_WARPS - 1) / SCAN_WARPS, 32 * SCAN_WARPS, 0, stream>>>(
-                digits, tiles, totals + pass * digits, counts);
-            HDS_CHECK_LAUNCH("scan_kernel");
-            scatter<<<tiles, SORT_THREADS, shared, stream>>>(n, source, shift, plan.digit_bits, tiles, counts, keys,
-                                                             rows);
+            if (plan.scan) {
+                scan_kernel<<<(digits + SCAN_WARPS - 1) / SCAN_WARPS, 32 * SCAN_WARPS, 0, stream>>>(digits, tiles,
+                                                                                                  counts);
+                HDS_CHECK_LAUNCH("scan_kernel");
+            }
+            scatter<<<tiles, SORT_THREADS, shared, stream>>>((int)n, source, shift, plan.digit_bits, tiles, plan.scan, counts,
+                                                             totals + pass * digits, pairs);
             HDS_CHECK_LAUNCH("scatter_kernel");
             return HDS_OK;
         };
         if (int rc = plan.rounds == MANY_ROUNDS ? run(histogram_kernel<MANY_ROUNDS>, scatter_kernel<MANY_ROUNDS>)
                                                 : run(histogram_kernel<SOME_ROUNDS>, scatter_kernel<SOME_ROUNDS>))
             return rc;
-        source.keys = keys;
-        source.rows = rows;
-        std::swap(keys, keys_other);
-        std::swap(rows, rows_other);
+        source.pairs = pairs;
+        std::swap(pairs, pairs_other);
     }
-    const uint32_t* sorted_keys = source.keys;
-    const int32_t* sorted_rows = source.rows;
+    const uint2* sorted = source.pairs;
 
     const int slabs = (channels + plan.slab - 1) / plan.slab;
     const int64_t threads = plan.chunks << plan.lanes_log2;
-    const dim3 sum_grid((unsigned)((threads + THREADS - 1) / THREADS), (unsigned)slabs);
+    const unsigned sum_grid = (unsigned)((threads + THREADS - 1) / THREADS * slabs);
     const dim3 join_grid((unsigned)((plan.chunks + JOIN_WORKERS - 1) / JOIN_WORKERS),
                          (unsigned)((channels + JOIN_COLUMNS - 1) / JOIN_COLUMNS));
     return with_variant([&](auto g, auto t, auto drop, auto add) -> int {
@@ -1028,7 +1151,7 @@ extern "C" int hds_embedding_backward(int64_t n, int64_t vocab, int channels, in
         if (int rc = with_vector(v, [&](auto width) -> int {
                 chunk_sum_kernel<G, T, decltype(width)::value, decltype(drop)::value, decltype(add)::value>
                     <<<sum_grid, THREADS, 0, stream>>>(n, (uint32_t)vocab, channels, plan.slab, plan.lanes_log2,
-                                                       plan.chunk, sorted_keys, sorted_rows,
+                                                       plan.chunk, slabs, sorted,
                                                        static_cast<const G*>(grad), factor,
                                                        below_last(drop_threshold), d, static_cast<T*>(grad_table), heads, tails, plan.stride);
                 HDS_CHECK_LAUNCH("chunk_sum_kernel");
@@ -1037,7 +1160,7 @@ extern "C" int hds_embedding_backward(int64_t n, int64_t vocab, int channels, in
             return rc;
         if (plan.chunks == 1) return HDS_OK;
         const auto join = [&](auto* kernel) -> int {
-            kernel<<<join_grid, THREADS, 0, stream>>>(n, (uint32_t)vocab, channels, plan.chunk, sorted_keys, heads,
+            kernel<<<join_grid, THREADS, 0, stream>>>(n, (uint32_t)vocab, channels, plan.chunk, sorted, heads,
                                                       tails, plan.stride, factor, static_cast<T*>(grad_table));
             HDS_CHECK_LAUNCH("join_kernel");
             return HDS_OK;

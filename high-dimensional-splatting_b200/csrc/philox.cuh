@@ -54,6 +54,8 @@ struct Numbers8 {
     }
 };
 
+// The numbers of group 2^32 group_high + group_low.  A group_high that is the same in every lane (a constant,
+// or made from blockIdx) takes two of the twenty products out of the lanes' work.
 __device__ __forceinline__ Numbers8 philox4x32_10(uint32_t group_low, uint32_t group_high, const Draw& d) {
     uint32_t x0 = group_low, x1 = group_high;
     uint32_t x2 = (uint32_t)d.offset, x3 = (uint32_t)(d.offset >> 32);
@@ -69,10 +71,6 @@ __device__ __forceinline__ Numbers8 philox4x32_10(uint32_t group_low, uint32_t g
         k1 += 0xBB67AE85u;
     }
     return Numbers8{{x0, x1, x2, x3}};
-}
-
-__device__ __forceinline__ Numbers8 philox4x32_10(uint64_t group, const Draw& d) {
-    return philox4x32_10((uint32_t)group, (uint32_t)(group >> 32), d);
 }
 
 // For the kernels' below_last; thresholds from 1 to 65536 (modulo 2^32).

@@ -341,6 +341,7 @@ enum {
     HDS_TYPE_I64 = 4
 };
 #define HDS_EMBEDDING_MAX_CHANNELS 32768
+#define HDS_EMBEDDING_MAX_DROPOUT (INT64_C(1) << 35) /* values of a lookup with dropout */
 int hds_embedding_forward(int64_t n, int64_t vocab, int channels, int table_type, const void* table, int ids_type,
                           const void* ids, int has_padding, int64_t padding_id, double scale, int drop_threshold,
                           uint64_t seed, uint64_t offset, const int64_t* draw, int out_type, void* out,

@@ -6,8 +6,16 @@ whether or not a bound is close."""
 from __future__ import annotations
 
 import math
+import multiprocessing.util
+import time
 
 import numpy as np
+
+# A spawned worker that sends tensors through a queue serves their file descriptors until it exits; the
+# parent may still be fetching them then.  A worker that imports this module stays a moment longer, before
+# its exit closes the socket they are fetched through (priority 0).
+if multiprocessing.current_process().name != "MainProcess":
+    multiprocessing.util.Finalize(None, time.sleep, args=(1.0,), exitpriority=100)
 
 # Tolerances from the build's north star: RGB within 1e-5 absolute, feature images within 1e-3
 # absolute, gradients within 1e-4 relative (every entry within 1e-4 of the tensor's largest

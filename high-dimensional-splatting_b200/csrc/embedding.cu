@@ -918,15 +918,20 @@ struct BackwardPlan {
     }
 };
 
-// Shared argument checks of both directions.
-int check_arguments(const char* what, int64_t n, int64_t vocab, int channels, int table_type, int value_type,
-                    int ids_type, double scale, int drop_threshold) {
+int check_sizes(const char* what, int64_t n, int64_t vocab, int64_t channels) {
     HDS_REQUIRE(n >= 0 && vocab >= 0 && channels >= 0, HDS_ERR_INVALID, "%s: negative size", what);
     // Row numbers are 32-bit, also of the last, partly empty, block.
     constexpr int64_t most = INT32_MAX - (1 << 20);
     HDS_REQUIRE(n <= most && vocab <= most && channels <= HDS_EMBEDDING_MAX_CHANNELS, HDS_ERR_TOO_LARGE,
-                "%s: n = %lld, vocab = %lld, channels = %d is too large", what, (long long)n, (long long)vocab,
-                channels);
+                "%s: n = %lld, vocab = %lld, channels = %lld is too large", what, (long long)n, (long long)vocab,
+                (long long)channels);
+    return HDS_OK;
+}
+
+// Shared argument checks of both directions.
+int check_arguments(const char* what, int64_t n, int64_t vocab, int64_t channels, int table_type, int value_type,
+                    int ids_type, double scale, int drop_threshold) {
+    if (int rc = check_sizes(what, n, vocab, channels)) return rc;
     HDS_REQUIRE(known_type(table_type) && (value_type == table_type || value_type == HDS_TYPE_F32),
                 HDS_ERR_UNSUPPORTED, "%s: values must be of the table's type or fp32", what);
     HDS_REQUIRE(ids_type == HDS_TYPE_I32 || ids_type == HDS_TYPE_I64, HDS_ERR_UNSUPPORTED,
@@ -965,14 +970,15 @@ int read_and_clear_embedding_status(int* status, cudaStream_t stream) {
 
 using namespace hds;
 
-extern "C" int hds_embedding_forward(int64_t n, int64_t vocab, int channels, int table_type, const void* table,
+extern "C" int hds_embedding_forward(int64_t n, int64_t vocab, int64_t columns, int table_type, const void* table,
                                      int ids_type, const void* ids, int has_padding, int64_t padding_id, double scale,
                                      int drop_threshold, uint64_t seed, uint64_t offset, const int64_t* draw,
                                      int out_type, void* out, hds_stream_t stream) {
     clear_error();
-    if (int rc = check_arguments("embedding", n, vocab, channels, table_type, out_type, ids_type, scale,
+    if (int rc = check_arguments("embedding", n, vocab, columns, table_type, out_type, ids_type, scale,
                                  drop_threshold))
         return rc;
+    const int channels = (int)columns;
     if (n == 0 || channels == 0) return HDS_OK;
     HDS_REQUIRE((table != nullptr || vocab == 0) && ids != nullptr && out != nullptr, HDS_ERR_INVALID,
                 "embedding: null pointer");
@@ -1031,19 +1037,23 @@ extern "C" int hds_embedding_forward(int64_t n, int64_t vocab, int channels, int
     });
 }
 
-extern "C" size_t hds_embedding_backward_scratch_bytes(int64_t n, int64_t vocab, int channels) {
+extern "C" size_t hds_embedding_backward_scratch_bytes(int64_t n, int64_t vocab, int64_t columns) {
+    // Sizes that hds_embedding_backward refuses need none.
+    if (check_sizes("embedding_backward", n, vocab, columns) != HDS_OK) return 0;
+    const int channels = (int)columns;
     return FewRowsPlan(n, vocab, channels).fits ? 0 : BackwardPlan(n, vocab, channels).bytes;
 }
 
-extern "C" int hds_embedding_backward(int64_t n, int64_t vocab, int channels, int grad_type, const void* grad,
+extern "C" int hds_embedding_backward(int64_t n, int64_t vocab, int64_t columns, int grad_type, const void* grad,
                                       int ids_type, const void* ids, int has_padding, int64_t padding_id,
                                       double scale, int drop_threshold, uint64_t seed, uint64_t offset,
                                       const int64_t* draw, int table_type, void* grad_table, int accumulate,
                                       void* scratch, size_t scratch_bytes, hds_stream_t stream) {
     clear_error();
-    if (int rc = check_arguments("embedding_backward", n, vocab, channels, table_type, grad_type, ids_type, scale,
+    if (int rc = check_arguments("embedding_backward", n, vocab, columns, table_type, grad_type, ids_type, scale,
                                  drop_threshold))
         return rc;
+    const int channels = (int)columns;
     HDS_REQUIRE(!accumulate || table_type == HDS_TYPE_F32, HDS_ERR_UNSUPPORTED,
                 "embedding_backward: only an fp32 gradient buffer can be added to");
     if (vocab == 0 || channels == 0) return HDS_OK;

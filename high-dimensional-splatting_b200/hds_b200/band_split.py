@@ -46,6 +46,25 @@ def band_reach_mask(means2D: torch.Tensor, radii: torch.Tensor, y0: int, y1: int
     return (radii > 0) & (v + reach >= float(y0 - 16)) & (v - reach < float(y1 + 16))
 
 
+def gather_rows(rows: torch.Tensor, ids: torch.Tensor) -> torch.Tensor:
+    """rows[ids], a fresh contiguous [M, C] tensor: on the GPU the codebook lookup's kernel."""
+    if rows.is_cuda:
+        from .gaussian_rasterizer import embedding
+
+        return embedding(rows, ids)
+    return rows[ids].contiguous()
+
+
+def add_rows(target: torch.Tensor, ids: torch.Tensor, rows: torch.Tensor) -> None:
+    """target[ids] += rows: on the GPU by the codebook lookup's gradient, one pass without atomics."""
+    if target.is_cuda:
+        from .gaussian_rasterizer import embedding_backward_into
+
+        embedding_backward_into(target, rows, ids)
+    else:
+        target.index_add_(0, ids, rows)
+
+
 class FeatureShards:
     """The feature table split over the group's ranks: by contiguous row blocks, or by an owner map.
 
@@ -104,7 +123,7 @@ class FeatureShards:
         when given, a contiguous [M, C] tensor)."""
         if self.world == 1:
             self._plan = None
-            return self.rows.detach()[self._local(ids)]
+            return gather_rows(self.rows.detach(), self._local(ids))
         if self.owner is None:
             # Sorted ids and contiguous owners keep every owner's requests in one slice of ids.
             own = torch.searchsorted(self._bounds, ids, right=True)
@@ -121,7 +140,7 @@ class FeatureShards:
         dist.all_to_all_single(wanted, grouped.contiguous(), output_split_sizes=recv, input_split_sizes=send,
                                group=self.group)
         local = self._local(wanted)
-        served = self.rows.detach()[local].contiguous()
+        served = gather_rows(self.rows.detach(), local)
         if out is not None and perm is None:
             got = out
         else:
@@ -156,7 +175,7 @@ class FeatureShards:
             wanted = torch.empty(sum(recv), dtype=ids.dtype, device=ids.device)
             dist.all_to_all_single(wanted, ids, output_split_sizes=recv, input_split_sizes=send, group=self.group)
             local = self._local(wanted)
-            served = self.rows.detach()[local].contiguous()
+            served = gather_rows(self.rows.detach(), local)
             got = torch.empty(ids.numel(), self.channels, dtype=served.dtype, device=ids.device)
             dist.all_to_all_single(got, served, output_split_sizes=send, input_split_sizes=recv, group=self.group)
         ids.record_stream(side)
@@ -174,20 +193,18 @@ class FeatureShards:
     def combine(self, ids: torch.Tensor, grads: torch.Tensor) -> None:
         """Adds grads ([M, C], rows of the ids of the last dispatch) into the owners' rows.grad."""
         if self.world == 1:
-            self.rows.grad.index_add_(0, self._local(ids), grads)
+            add_rows(self.rows.grad, self._local(ids), grads.contiguous())
             return
         send, recv, local, perm = self._plan
         outgoing = grads if perm is None else grads[perm]
         back = torch.empty(sum(recv), self.channels, dtype=grads.dtype, device=grads.device)
         dist.all_to_all_single(back, outgoing.contiguous(), output_split_sizes=recv, input_split_sizes=send,
                                group=self.group)
-        # Each requester's ids are distinct, so within its slice every row is added once: a gather, an
-        # add and a scatter per slice instead of one float atomic per element.
-        g, off = self.rows.grad, 0
+        # Slice by slice, in rank order: each requester's ids are distinct, so a row's sum has one order.
+        off = 0
         for k in recv:
             if k:
-                idx = local[off:off + k]
-                g[idx] = g[idx] + back[off:off + k]
+                add_rows(self.rows.grad, local[off:off + k], back[off:off + k])
             off += k
 
 

@@ -471,14 +471,17 @@ def drop_threshold(p: float) -> int:
 _LOW64 = 0xFFFFFFFFFFFFFFFF
 
 
-def _draw(seed, offset, draw, device):
-    """(seed, offset, draw pointer): the two numbers modulo 2^64, or the address of an int64 [2] tensor
-    that holds them."""
+def _draw(p, seed, offset, draw, device):
+    """(threshold, seed, offset, draw pointer): the two numbers modulo 2^64, or the address of an int64 [2]
+    tensor that holds them."""
+    if p == 0.0:
+        return 0, 0, 0, None
+    threshold = drop_threshold(p)
     if draw is None:
-        return int(seed) & _LOW64, int(offset) & _LOW64, None
+        return threshold, int(seed) & _LOW64, int(offset) & _LOW64, None
     if draw.dtype != torch.int64 or draw.shape != (2,) or not draw.is_contiguous() or draw.device != device:
         raise RuntimeError("draw must be a contiguous int64 tensor [2] (seed, offset) on the input's device")
-    return 0, 0, draw.data_ptr()
+    return threshold, 0, 0, draw.data_ptr()
 
 
 def _check_lookup(table_dtype, value_dtype, ids, device, padding_id):
@@ -510,8 +513,7 @@ def embedding(table, ids, dtype=None, scale: float = 1.0, padding_id: int | None
     dtype = dtype or table.dtype
     dev = table.device
     _check_lookup(table.dtype, dtype, ids, dev, padding_id)
-    threshold = drop_threshold(dropout_p)
-    seed, offset, draw_ptr = _draw(seed, offset, draw, dev)
+    threshold, seed, offset, draw_ptr = _draw(dropout_p, seed, offset, draw, dev)
     v, c = table.shape
     out = torch.empty(*ids.shape, c, dtype=dtype, device=dev)
     with on_device(dev):
@@ -528,8 +530,7 @@ def _embedding_backward(grad, ids, grad_table, accumulate, scale, padding_id, dr
     if grad.device != dev or grad.shape != (*ids.shape, c):
         raise RuntimeError(f"grad must be {(*ids.shape, c)} on the table's device")
     _check_lookup(grad_table.dtype, grad.dtype, ids, dev, padding_id)
-    threshold = drop_threshold(dropout_p)
-    seed, offset, draw_ptr = _draw(seed, offset, draw, dev)
+    threshold, seed, offset, draw_ptr = _draw(dropout_p, seed, offset, draw, dev)
     n = ids.numel()
     need = lib.hds_embedding_backward_scratch_bytes(n, v, c)
     scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
@@ -569,9 +570,8 @@ def dropout(x, p: float, seed: int = 0, offset: int = 0, rows: bool = False, dra
         raise RuntimeError("x must be float32, bfloat16 or float16")
     if rows and x.dim() == 0:
         raise RuntimeError("dropping whole rows needs at least one dimension")
-    threshold = drop_threshold(p)
     dev = x.device
-    seed, offset, draw_ptr = _draw(seed, offset, draw, dev)
+    threshold, seed, offset, draw_ptr = _draw(p, seed, offset, draw, dev)
     y = torch.empty_like(x)
     n = x.numel()
     c = x.shape[-1] if rows else 1

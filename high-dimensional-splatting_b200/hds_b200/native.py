@@ -57,10 +57,10 @@ SIGNATURES = {
     "hds_densify_stats": [c_int, P, P, c_int, c_int, P, P, P, S],
     "hds_densify_apply": [c_int, c_int, c_int, ctypes.POINTER(c_int), c_int, c_int, c_float, P, P, P, P, P, P, P, P,
                           P, S],
-    "hds_embedding_forward": [c_int64, c_int64, c_int, c_int, P, c_int, P, c_int, c_int64, c_double, c_int, c_uint64,
+    "hds_embedding_forward": [c_int64, c_int64, c_int64, c_int, P, c_int, P, c_int, c_int64, c_double, c_int, c_uint64,
                               c_uint64, P, c_int, P, S],
-    "hds_embedding_backward_scratch_bytes": [c_int64, c_int64, c_int],
-    "hds_embedding_backward": [c_int64, c_int64, c_int, c_int, P, c_int, P, c_int, c_int64, c_double, c_int, c_uint64,
+    "hds_embedding_backward_scratch_bytes": [c_int64, c_int64, c_int64],
+    "hds_embedding_backward": [c_int64, c_int64, c_int64, c_int, P, c_int, P, c_int, c_int64, c_double, c_int, c_uint64,
                                c_uint64, P, c_int, P, c_int, P, c_size_t, S],
     "hds_dropout": [c_int64, c_int64, c_int, P, c_int, c_int, c_uint64, c_uint64, P, P, S],
     "hds_device_status": [ctypes.POINTER(c_int), S],

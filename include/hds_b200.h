@@ -342,12 +342,12 @@ enum {
 };
 #define HDS_EMBEDDING_MAX_CHANNELS 32768
 #define HDS_EMBEDDING_MAX_DROPOUT (INT64_C(1) << 35) /* values of a lookup with dropout */
-int hds_embedding_forward(int64_t n, int64_t vocab, int channels, int table_type, const void* table, int ids_type,
+int hds_embedding_forward(int64_t n, int64_t vocab, int64_t channels, int table_type, const void* table, int ids_type,
                           const void* ids, int has_padding, int64_t padding_id, double scale, int drop_threshold,
                           uint64_t seed, uint64_t offset, const int64_t* draw, int out_type, void* out,
                           hds_stream_t stream);
-size_t hds_embedding_backward_scratch_bytes(int64_t n, int64_t vocab, int channels);
-int hds_embedding_backward(int64_t n, int64_t vocab, int channels, int grad_type, const void* grad, int ids_type,
+size_t hds_embedding_backward_scratch_bytes(int64_t n, int64_t vocab, int64_t channels);
+int hds_embedding_backward(int64_t n, int64_t vocab, int64_t channels, int grad_type, const void* grad, int ids_type,
                            const void* ids, int has_padding, int64_t padding_id, double scale, int drop_threshold,
                            uint64_t seed, uint64_t offset, const int64_t* draw, int table_type, void* grad_table,
                            int accumulate, void* scratch, size_t scratch_bytes, hds_stream_t stream);

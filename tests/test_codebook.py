@@ -68,6 +68,9 @@ INVALID, UNSUPPORTED, SCRATCH, TOO_LARGE = 1, 2, 4, 5
     (forward, dict(n=2**31), TOO_LARGE, "too large"),
     (forward, dict(vocab=2**31), TOO_LARGE, "too large"),
     (forward, dict(channels=32769), TOO_LARGE, "too large"),
+    (forward, dict(channels=2**32 + 8), TOO_LARGE, "too large"),
+    (forward, dict(n=2**31 - 2**21, channels=32768, drop=1), TOO_LARGE, "dropout of"),
+    (backward, dict(n=2**31 - 2**21, channels=32768, drop=1), TOO_LARGE, "dropout of"),
     (forward, dict(table_type=I32), UNSUPPORTED, "table's type"),
     (forward, dict(table_type=BF16, out_type=F16), UNSUPPORTED, "table's type"),
     (forward, dict(table_type=F32, out_type=BF16), UNSUPPORTED, "table's type"),

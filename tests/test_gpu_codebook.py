@@ -516,3 +516,29 @@ def test_codebook_features_through_the_rasterizer():
     # carry over (1e-4 of the largest entry is the suite's bound for the blend's gradients).
     want, bound = plain.table_gradient(as64(dense_grad), ids.cpu().numpy(), vocab, p=0.1, **how)
     assert np.abs(as64(got) - want).max() <= bound.max() + 1e-4 * np.abs(want).max()
+
+
+@pytest.mark.parametrize("c", [64, 50])
+def test_feature_shards_rows(c):
+    """The rows of a feature shard leave and arrive through the lookup and its gradient: bit for bit what
+    indexing gives."""
+    from hds_b200.band_split import FeatureShards, add_rows, gather_rows
+
+    rng = np.random.default_rng(8)
+    table = make_values(rng, (5000, c), torch.float32)
+    ids = torch.from_numpy(np.sort(rng.choice(5000, 1700, replace=False))).cuda()
+    assert torch.equal(gather_rows(table, ids), table[ids])
+    target, rows = make_values(rng, (5000, c), torch.float32), make_values(rng, (1700, c), torch.float32)
+    want = target.clone()
+    want[ids] = want[ids] + rows
+    add_rows(target, ids, rows)
+    assert torch.equal(target, want)
+    for owner in (None, torch.zeros(5000, dtype=torch.int64)):
+        shards = FeatureShards(5000, c, 0, 1, "cuda", init=lambda *a: table, owner=owner)
+        assert torch.equal(shards.dispatch(ids), table[ids])
+        shards.combine(ids, rows)
+        shards.combine(ids, rows)
+        want = torch.zeros_like(table)
+        want[ids] = rows + rows
+        assert torch.equal(shards.rows.grad, want)
+        assert shards.dispatch(ids[:0]).shape == (0, c)

@@ -28,9 +28,10 @@ constexpr int BLOCK_GROUPS = BLOCK_ELEMENTS / 8;
 template <typename T, int V>
 __device__ __forceinline__ Vec<T, V> load_up_to(const T* x, int64_t e, int64_t n) {
     if (e + V <= n) return load_once<T, V>(x + e);
-    Vec<T, V> v;
-    for (int j = 0; j < V; j++) v.set(j, e + j < n ? to_float(x[e + j]) : 0.0f);
-    return v;
+    float v[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) v[j] = e + j < n ? to_float(x[e + j]) : 0.0f;
+    return Vec<T, V>::pack(v);
 }
 
 template <typename T, int V>
@@ -67,13 +68,13 @@ __global__ void __launch_bounds__(DROPOUT_THREADS) dropout_kernel(int64_t n, con
         for (int k = 0; k < STEPS; k++) {
             const int at = (k * 32 + lane) * V;
             const uint32_t mine = V == 8 ? 0 : __shfl_sync(FULL_MASK, bits, at >> 3) >> (at & 7);
-            Vec<T, V> r;
+            float r[V];
 #pragma unroll
             for (int j = 0; j < V; j++) {
                 const bool kept = V == 8 ? numbers.kept(j, last) : ((mine >> j) & 1u) != 0;
-                r.set(j, kept ? v[t][k].get(j) * factor : 0.0f);
+                r[j] = kept ? v[t][k].get(j) * factor : 0.0f;
             }
-            store_up_to<T, V>(y, warp_base + t * TILE_ELEMENTS + at, n, r);
+            store_up_to<T, V>(y, warp_base + t * TILE_ELEMENTS + at, n, Vec<T, V>::pack(r));
         }
     }
 }
@@ -132,10 +133,10 @@ __global__ void __launch_bounds__(DROPOUT_THREADS) dropout_rows_kernel(int64_t n
     for (int t = 0; t < TILES; t++)
 #pragma unroll
         for (int k = 0; k < STEPS; k++) {
-            Vec<T, V> r;
+            float r[V];
 #pragma unroll
-            for (int j = 0; j < V; j++) r.set(j, (keep[t][k] >> j) & 1u ? v[t][k].get(j) * factor : 0.0f);
-            store_up_to<T, V>(y, warp_base + t * TILE_ELEMENTS + (k * 32 + lane) * V, n, r);
+            for (int j = 0; j < V; j++) r[j] = (keep[t][k] >> j) & 1u ? v[t][k].get(j) * factor : 0.0f;
+            store_up_to<T, V>(y, warp_base + t * TILE_ELEMENTS + (k * 32 + lane) * V, n, Vec<T, V>::pack(r));
         }
 }
 

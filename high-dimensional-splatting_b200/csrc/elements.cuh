@@ -28,6 +28,18 @@ __device__ __forceinline__ bf16 from_float<bf16>(float x) { return __float2bfloa
 template <>
 __device__ __forceinline__ f16 from_float<f16>(float x) { return __float2half_rn(x); }
 
+// Two elements in a word, the first in its lower half; one conversion instruction for both.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float low, float high) {
+    if constexpr (std::is_same<T, bf16>::value) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(low, high);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        const __half2 v = __floats2half2_rn(low, high);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
+
 // V elements moved as one vector (V = 8, 4, 2 or 1): 32 bytes at most, one 256-bit access of sm_100.
 template <typename T, int V>
 struct Vec {
@@ -43,21 +55,20 @@ struct Vec {
             return to_float(*reinterpret_cast<const T*>(&h));
         }
     }
-    // In the order of k: the lower half of a word clears the upper.
-    __device__ __forceinline__ void set(int k, float x) {
+    // The vector of V floats, each rounded to nearest.
+    static __device__ __forceinline__ Vec pack(const float* x) {
+        Vec r;
         if constexpr (sizeof(T) == 4) {
-            w[k] = __float_as_uint(x);
+#pragma unroll
+            for (int k = 0; k < V; k++) r.w[k] = __float_as_uint(x[k]);
+        } else if constexpr (V == 1) {
+            const T v = from_float<T>(x[0]);
+            r.w[0] = *reinterpret_cast<const uint16_t*>(&v);
         } else {
-            const T v = from_float<T>(x);
-            const uint32_t h = *reinterpret_cast<const uint16_t*>(&v);
-            w[k / 2] = k % 2 == 0 ? h : (w[k / 2] | (h << 16));
+#pragma unroll
+            for (int k = 0; k < V; k += 2) r.w[k / 2] = pack_pair<T>(x[k], x[k + 1]);
         }
-    }
-    __device__ __forceinline__ void clear(int k) {
-        if constexpr (sizeof(T) == 4)
-            w[k] = 0;
-        else
-            w[k / 2] &= k % 2 == 0 ? 0xffff0000u : 0xffffu;
+        return r;
     }
 };
 

@@ -115,11 +115,12 @@ __global__ void __launch_bounds__(THREADS, DROP ? 8 : 1) lookup_rows_kernel(int 
     for (int p = 0; p < PASSES; p++) {
         Numbers8 numbers{};
         if (DROP) numbers = philox4x32_10(group + (uint32_t)(p * rows_at_once * vectors), 0, draw);
-        Vec<O, V> result;
+        float result[V];
 #pragma unroll
-        for (int j = 0; j < V; j++) result.set(j, !DROP || numbers.kept(j, last) ? v[p].get(j) * factor : 0.0f);
-        if (from[p] < 0) result = Vec<O, V>{};
-        if (p * rows_at_once < left) store<O, V>(to + p * step, result);
+        for (int j = 0; j < V; j++) result[j] = !DROP || numbers.kept(j, last) ? v[p].get(j) * factor : 0.0f;
+        Vec<O, V> packed = Vec<O, V>::pack(result);
+        if (from[p] < 0) packed = Vec<O, V>{};
+        if (p * rows_at_once < left) store<O, V>(to + p * step, packed);
     }
 }
 
@@ -169,20 +170,20 @@ __global__ void __launch_bounds__(THREADS) lookup_groups_kernel(int n, int chann
         }
         Numbers8 numbers{};
         if (DROP) numbers = philox4x32_10((uint32_t)group0 + g, 0, draw);
-        Vec<O, 8> r;
+        float r[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-            r.set(j, !DROP || numbers.kept(j, last) ? v[j / V].get(j % V) * factor : 0.0f);
+        for (int j = 0; j < 8; j++) r[j] = !DROP || numbers.kept(j, last) ? v[j / V].get(j % V) * factor : 0.0f;
         if (there != 0xffu) {
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (!((there >> j) & 1u)) r.clear(j);
+            for (int j = 0; j < 8; j++) r[j] = (there >> j) & 1u ? r[j] : 0.0f;
         }
-        if (whole && first + 8 <= total)
-            store<O, 8>(out + first, r);
-        else
+        if (whole && first + 8 <= total) {
+            store<O, 8>(out + first, Vec<O, 8>::pack(r));
+        } else {
+#pragma unroll
             for (int j = 0; j < 8; j++)
-                if (first + j < total) out[first + j] = from_float<O>(r.get(j));
+                if (first + j < total) out[first + j] = from_float<O>(r[j]);
+        }
     }
 }
 
@@ -239,11 +240,10 @@ struct PairSource {
     }
 };
 
-// counts[digit][tile] and totals[digit] (cleared by the caller; integer adds, so their order is no matter).
+// counts[digit][tile].
 template <int ROUNDS>
 __global__ void __launch_bounds__(SORT_THREADS) histogram_kernel(int n, PairSource source, int shift, int bits,
-                                                                 int tiles, uint32_t* __restrict__ counts,
-                                                                 uint32_t* __restrict__ totals) {
+                                                                 int tiles, uint32_t* __restrict__ counts) {
     __shared__ uint32_t hist[MAX_DIGITS];
     const int digits = 1 << bits;
     for (int d = threadIdx.x; d < digits; d += SORT_THREADS) hist[d] = 0;
@@ -261,22 +261,20 @@ __global__ void __launch_bounds__(SORT_THREADS) histogram_kernel(int n, PairSour
         if (valid && lane == __ffs(peers) - 1) atomicAdd(&hist[d], __popc(peers));
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < digits; d += SORT_THREADS) {
-        const uint32_t c = hist[d];
-        counts[(int64_t)d * tiles + blockIdx.x] = c;
-        if (c) atomicAdd(&totals[d], c);
-    }
+    for (int d = threadIdx.x; d < digits; d += SORT_THREADS) counts[(int64_t)d * tiles + blockIdx.x] = hist[d];
 }
 
 // A scatter block sums the counts of the tiles before its own itself where that takes few loads: a thread a
 // digit for 16 tiles at most, a warp a digit for 160 tiles and 256 digits at most.
 constexpr int FEW_TILES = 16, SOME_TILES = 160, SOME_DIGIT_BITS = 8;
 
-// counts[digit][tile] -> how many keys of that digit the tiles before have.  A warp per digit.
+// counts[digit][tile] -> how many keys of that digit the tiles before have, and totals[digit].  A warp per
+// digit.
 constexpr int SCAN_WARPS = 8;
 
 __global__ void __launch_bounds__(32 * SCAN_WARPS) scan_kernel(int digits, int tiles,
-                                                               uint32_t* __restrict__ counts) {
+                                                               uint32_t* __restrict__ counts,
+                                                               uint32_t* __restrict__ totals) {
     const int lane = threadIdx.x & 31, digit = blockIdx.x * SCAN_WARPS + (threadIdx.x >> 5);
     if (digit >= digits) return;
     uint32_t base = 0;
@@ -298,6 +296,7 @@ __global__ void __launch_bounds__(32 * SCAN_WARPS) scan_kernel(int digits, int t
             base += __shfl_sync(FULL_MASK, x, 31);
         }
     }
+    if (lane == 0) totals[digit] = base;
 }
 
 // Each warp ranks its own consecutive keys into a count table of its own; a scan over the digits and the
@@ -305,7 +304,7 @@ __global__ void __launch_bounds__(32 * SCAN_WARPS) scan_kernel(int digits, int t
 // digits.  (Stored straight from the registers, each of a warp's pairs is a memory access of its own, and
 // the scatter of 1.18M pairs took 20 us instead of SCATTER_US.)
 inline size_t scatter_shared_bytes(int digits, int rounds) {
-    return (size_t)digits * (sizeof(uint32_t) + 2 * SORT_WARPS) + (size_t)rounds * SORT_THREADS * sizeof(uint2);
+    return (size_t)digits * (2 * sizeof(uint32_t) + 2 * SORT_WARPS) + (size_t)rounds * SORT_THREADS * sizeof(uint2);
 }
 
 template <int ROUNDS>
@@ -320,7 +319,8 @@ __global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(int n, PairSource
     __shared__ uint2 s_total[SORT_WARPS];
     const int digits = 1 << bits, own = max(1, digits / SORT_THREADS);
     uint32_t* s_move = reinterpret_cast<uint32_t*>(s_pair + TILE);           // [digits]: output - tile position
-    uint16_t* s_warp = reinterpret_cast<uint16_t*>(s_move + digits);         // [warps][digits]
+    uint32_t* s_all = s_move + digits;                                       // [digits]
+    uint16_t* s_warp = reinterpret_cast<uint16_t*>(s_all + digits);          // [warps][digits]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int tile = blockIdx.x * TILE;
     const int base = tile + warp * (32 * ROUNDS) + lane;
@@ -328,33 +328,39 @@ __global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(int n, PairSource
     uint2 pair[ROUNDS];
     uint16_t rank[ROUNDS];
     source.load<ROUNDS>(base, 32, n, pair);
-    // s_move for now: the digit's keys in the tiles before this one.
+    // The digit's keys in all tiles, and (s_move for now) in the tiles before this one.
     if (scanned) {
-        for (int d = tid; d < digits; d += SORT_THREADS) s_move[d] = counts[(int64_t)d * tiles + blockIdx.x];
+        for (int d = tid; d < digits; d += SORT_THREADS) {
+            s_move[d] = counts[(int64_t)d * tiles + blockIdx.x];
+            s_all[d] = totals[d];
+        }
     } else if (tiles <= FEW_TILES) {
         for (int d = tid; d < digits; d += SORT_THREADS) {
-            uint32_t before = 0;
+            uint32_t before = 0, all = 0;
 #pragma unroll
-            for (int t = 0; t < FEW_TILES; t++) before += t < (int)blockIdx.x ? counts[(int64_t)d * tiles + t] : 0;
+            for (int t = 0; t < FEW_TILES; t++) {
+                const uint32_t c = t < tiles ? counts[(int64_t)d * tiles + t] : 0;
+                before += t < (int)blockIdx.x ? c : 0;
+                all += c;
+            }
             s_move[d] = before;
+            s_all[d] = all;
         }
     } else {
 #pragma unroll 4
         for (int d = warp; d < digits; d += SORT_WARPS) {
-            uint32_t before = 0;
+            uint32_t before = 0, all = 0;
 #pragma unroll
-            for (int t = lane; t < SOME_TILES; t += 32)
-                before += t < (int)blockIdx.x ? counts[(int64_t)d * tiles + t] : 0;
+            for (int t = lane; t < SOME_TILES; t += 32) {
+                const uint32_t c = t < tiles ? counts[(int64_t)d * tiles + t] : 0;
+                before += t < (int)blockIdx.x ? c : 0;
+                all += c;
+            }
             before = __reduce_add_sync(FULL_MASK, before);
+            all = __reduce_add_sync(FULL_MASK, all);
             if (lane == 0) s_move[d] = before;
+            if (lane == 0) s_all[d] = all;
         }
-    }
-    uint32_t everywhere[OWN], sum_everywhere = 0;  // the digit's keys in all tiles
-#pragma unroll
-    for (int h = 0; h < OWN; h++) {
-        const int d = tid * own + h;
-        everywhere[h] = h < own && d < digits ? totals[d] : 0;
-        sum_everywhere += everywhere[h];
     }
     for (int i = tid; i < digits * SORT_WARPS / 2; i += SORT_THREADS) reinterpret_cast<uint32_t*>(s_warp)[i] = 0;
     __syncthreads();
@@ -371,10 +377,12 @@ __global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(int n, PairSource
     }
     __syncthreads();
     // Where each digit, and in it each warp, starts in the tile.
-    uint32_t total[OWN], sum = 0;
+    uint32_t total[OWN], sum = 0, everywhere[OWN], sum_everywhere = 0;
 #pragma unroll
     for (int h = 0; h < OWN; h++) {
         const int d = tid * own + h;
+        everywhere[h] = h < own && d < digits ? s_all[d] : 0;
+        sum_everywhere += everywhere[h];
         total[h] = 0;
         if (h < own && d < digits)
 #pragma unroll
@@ -440,11 +448,12 @@ constexpr int ROWS_AHEAD = 4;    // rows loaded before the first is added
 
 template <typename T, int V, bool ACCUMULATE>
 __device__ __forceinline__ void store_sum(T* p, const float* sum, float factor) {
-    Vec<T, V> r;
-    if (ACCUMULATE) r = load_once<T, V>(p);
+    Vec<T, V> old;
+    if (ACCUMULATE) old = load_once<T, V>(p);
+    float r[V];
 #pragma unroll
-    for (int j = 0; j < V; j++) r.set(j, ACCUMULATE ? fmaf(factor, sum[j], r.get(j)) : factor * sum[j]);
-    store<T, V>(p, r);
+    for (int j = 0; j < V; j++) r[j] = ACCUMULATE ? fmaf(factor, sum[j], old.get(j)) : factor * sum[j];
+    store<T, V>(p, Vec<T, V>::pack(r));
 }
 
 // Three blocks an SM (85 registers a thread) take 1.18M x 512 with dropout from 598 to 532 us; narrow vectors
@@ -912,7 +921,7 @@ struct BackwardPlan {
         pairs_b = pairs_a + align256(nn * sizeof(uint2));
         counts = pairs_b + align256(nn * sizeof(uint2));
         totals = counts + align256(((size_t)tiles << digit_bits) * 4);
-        heads = totals + align256(((size_t)passes << digit_bits) * 4);
+        heads = totals + align256(((size_t)1 << digit_bits) * 4);
         tails = heads + align256((size_t)chunks * stride * 4);
         bytes = tails + align256((size_t)chunks * stride * 4);
     }
@@ -1120,7 +1129,6 @@ extern "C" int hds_embedding_backward(int64_t n, int64_t vocab, int64_t columns,
     auto* heads = reinterpret_cast<float*>(s + plan.heads);
     auto* tails = reinterpret_cast<float*>(s + plan.tails);
     const int digits = 1 << plan.digit_bits, tiles = (int)plan.tiles;
-    HDS_CHECK_CUDA(cudaMemsetAsync(totals, 0, (size_t)plan.passes * digits * 4, stream));
     PairSource source{nullptr, id};
     for (int pass = 0; pass < plan.passes; pass++) {
         const int shift = pass * plan.digit_bits;
@@ -1129,16 +1137,15 @@ extern "C" int hds_embedding_backward(int64_t n, int64_t vocab, int64_t columns,
             if (shared > DEFAULT_SHARED_BYTES)
                 HDS_CHECK_CUDA(cudaFuncSetAttribute(scatter, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                     (int)scatter_shared_bytes(MAX_DIGITS, plan.rounds)));
-            histogram<<<tiles, SORT_THREADS, 0, stream>>>((int)n, source, shift, plan.digit_bits, tiles, counts,
-                                                          totals + pass * digits);
+            histogram<<<tiles, SORT_THREADS, 0, stream>>>((int)n, source, shift, plan.digit_bits, tiles, counts);
             HDS_CHECK_LAUNCH("histogram_kernel");
             if (plan.scan) {
-                scan_kernel<<<(digits + SCAN_WARPS - 1) / SCAN_WARPS, 32 * SCAN_WARPS, 0, stream>>>(digits, tiles,
-                                                                                                  counts);
+                scan_kernel<<<(digits + SCAN_WARPS - 1) / SCAN_WARPS, 32 * SCAN_WARPS, 0, stream>>>(
+                    digits, tiles, counts, totals);
                 HDS_CHECK_LAUNCH("scan_kernel");
             }
             scatter<<<tiles, SORT_THREADS, shared, stream>>>((int)n, source, shift, plan.digit_bits, tiles, plan.scan, counts,
-                                                             totals + pass * digits, pairs);
+                                                             totals, pairs);
             HDS_CHECK_LAUNCH("scatter_kernel");
             return HDS_OK;
         };

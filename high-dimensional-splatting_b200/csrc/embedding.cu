@@ -3,7 +3,8 @@
 // elements in the same pass (philox.cuh): f = scale / kept share, dropped elements 0 in both directions.
 //
 // Lookup.  One pass: the output is written once, the table's rows come from the L2 when the codebook is
-// smaller than it.
+// smaller than it.  Bound by the writes: 1.18M x 512 fp32 in 400 us, 2.4 GB at 6.1 TB/s (0.93 of the measured
+// copy rate); with dropout 424 us, where the generator's integer work begins to count.
 //
 // Gradient.  The rows are put in codeword order by a stable radix sort of (id, row number), and each
 // codeword's rows are summed in that order in fp32: no float atomics, so a call's result does not depend
@@ -89,11 +90,13 @@ constexpr int WIDE_BYTES = V * (sizeof(O) > sizeof(T) ? (int)sizeof(O) : (int)si
 template <typename T, typename O, int V>
 constexpr int LOOKUP_PASSES = 64 / WIDE_BYTES<T, O, V> < 8 ? 64 / WIDE_BYTES<T, O, V> : 8;
 
+// With dropout the generator's integer work is what the warps wait for: all the blocks that fit (32 registers a
+// thread) take 1.18M x 512 from 461 to 424 us.
 template <typename T, typename O, int V, bool DROP>
-__global__ void __launch_bounds__(THREADS, DROP ? 8 : 1) lookup_rows_kernel(int n, int channels, int vectors, int rows_at_once,
-                                                              Divider vectors_of, const T* __restrict__ table, Ids ids,
-                                                              float factor, uint32_t last, Draw draw,
-                                                              O* __restrict__ out) {
+__global__ void __launch_bounds__(THREADS, DROP ? 8 : 1)
+    lookup_rows_kernel(int n, int channels, int vectors, int rows_at_once, Divider vectors_of,
+                       const T* __restrict__ table, Ids ids, float factor, uint32_t last, Draw draw,
+                       O* __restrict__ out) {
     static_assert(V == 8 || !DROP, "a thread draws for whole groups of eight");
     constexpr int PASSES = LOOKUP_PASSES<T, O, V>;
     if (DROP) draw = resolve(draw);
@@ -128,7 +131,7 @@ __global__ void __launch_bounds__(THREADS, DROP ? 8 : 1) lookup_rows_kernel(int 
 // Eight rows are whole groups, so a block takes `eights` times eight rows, group by group: one generator
 // call still serves eight elements, an id eight of its row's, and the output is one vector.  A group's elements
 // come from the table in vectors of V, from two rows at most (any number when rows are narrower than a
-// group).  (With a thread per element 1.18M x 75 fp32 took 174 us, GROUPS_US like this.)
+// group).  (With a thread per element 1.18M x 75 fp32 took 174 us, 109 like this.)
 template <typename T, typename O, int V, bool DROP>
 __global__ void __launch_bounds__(THREADS) lookup_groups_kernel(int n, int channels, int eights, Divider rows_of,
                                                                 const T* __restrict__ table, Ids ids, float factor,
@@ -138,17 +141,16 @@ __global__ void __launch_bounds__(THREADS) lookup_groups_kernel(int n, int chann
     const int groups = eights * channels;  // of the block
     const int row0 = blockIdx.x * 8 * eights;
     const uint64_t group0 = (uint64_t)blockIdx.x * groups;
-    const int64_t total = (int64_t)n * channels;
+    O* to = out + group0 * 8;
+    const int here = (int)min((int64_t)groups * 8, ((int64_t)n - row0) * channels);  // elements of the block
     const auto row_of = [&](uint32_t e) -> int {
         return rows_of.d != 0 ? (int)rows_of.quotient(e) : (int)(e / (uint32_t)channels);
     };
-    for (int g = threadIdx.x; g < groups; g += THREADS) {
-        const int64_t first = (int64_t)(group0 + g) * 8;
-        if (first >= total) break;
+    for (int e0 = 8 * threadIdx.x; e0 < here; e0 += 8 * THREADS) {
         Vec<T, V> v[8 / V];
         uint32_t there = 0;  // bit j: element j comes from the table (its first row in the place of no row)
         if (channels >= 8) {
-            const int q = row_of(8 * g), col = 8 * g - q * channels, left = channels - col;
+            const int q = row_of(e0), col = e0 - q * channels, left = channels - col;
             int from[2];
             ids.rows<2>(row0 + q, 1, n, from);
             const uint32_t in_a = left >= 8 ? 0xffu : (1u << left) - 1u;
@@ -160,16 +162,16 @@ __global__ void __launch_bounds__(THREADS) lookup_groups_kernel(int n, int chann
         } else {
 #pragma unroll
             for (int k = 0; k < 8 / V; k++) {
-                const int q = row_of(8 * g + k * V);
+                const int q = row_of(e0 + k * V);
                 int from[1];
                 ids.rows<1>(row0 + q, 1, n, from);
                 if (from[0] >= 0) there |= ((1u << V) - 1u) << (k * V);
                 v[k] = load_shared_data<T, V>(table + (int64_t)max(from[0], 0) * channels +
-                                              (8 * g + k * V - q * channels));
+                                              (e0 + k * V - q * channels));
             }
         }
         Numbers8 numbers{};
-        if (DROP) numbers = philox4x32_10((uint32_t)group0 + g, 0, draw);
+        if (DROP) numbers = philox4x32_10((uint32_t)group0 + e0 / 8, 0, draw);
         float r[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) r[j] = !DROP || numbers.kept(j, last) ? v[j / V].get(j % V) * factor : 0.0f;
@@ -177,12 +179,12 @@ __global__ void __launch_bounds__(THREADS) lookup_groups_kernel(int n, int chann
 #pragma unroll
             for (int j = 0; j < 8; j++) r[j] = (there >> j) & 1u ? r[j] : 0.0f;
         }
-        if (whole && first + 8 <= total) {
-            store<O, 8>(out + first, Vec<O, 8>::pack(r));
+        if (whole && e0 + 8 <= here) {
+            store<O, 8>(to + e0, Vec<O, 8>::pack(r));
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (first + j < total) out[first + j] = from_float<O>(r[j]);
+                if (e0 + j < here) to[e0 + j] = from_float<O>(r[j]);
         }
     }
 }
@@ -204,8 +206,9 @@ __device__ __forceinline__ uint32_t lanes_alike(uint32_t digit, int bits, bool v
 }
 
 // Digits of up to 11 bits: one pass for codebooks below 2048 rows, two below 4M.  A pass is a histogram
-// per tile, a scan that turns the digit-major counts into output positions, and a scatter that ranks the
-// tile's keys.  The first pass reads the ids themselves.  No block waits for another.
+// per tile and a scatter that ranks the tile's keys, with a scan of the counts between them where they are
+// many.  The first pass reads the ids themselves.  No block waits for another.  Bound by latency: the passes
+// of 1.18M ids of 8192 codewords take 45 us together, 12% of the gradient's time at 512 channels.
 constexpr int SORT_THREADS = 512;
 constexpr int SORT_WARPS = SORT_THREADS / 32;
 // Keys per thread: 16 (a tile is 8192 keys) when that still gives every SM a tile, else 4.
@@ -302,7 +305,7 @@ __global__ void __launch_bounds__(32 * SCAN_WARPS) scan_kernel(int digits, int t
 // Each warp ranks its own consecutive keys into a count table of its own; a scan over the digits and the
 // warps places the tile's pairs in shared memory in sorted order, from where they go out in runs of equal
 // digits.  (Stored straight from the registers, each of a warp's pairs is a memory access of its own, and
-// the scatter of 1.18M pairs took 20 us instead of SCATTER_US.)
+// the scatter of 1.18M pairs took 20 us instead of 12.)
 inline size_t scatter_shared_bytes(int digits, int rounds) {
     return (size_t)digits * (2 * sizeof(uint32_t) + 2 * SORT_WARPS) + (size_t)rounds * SORT_THREADS * sizeof(uint2);
 }
@@ -442,7 +445,8 @@ __global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(int n, PairSource
 // group of 1 to 32 lanes with 8 columns each, adds up one chunk's rows in registers.  A codeword that
 // begins and ends inside the chunk goes straight to the table.  The sum of a codeword that began in an
 // earlier chunk is the chunk's head, that of one that goes on into the next its tail; join_kernel adds a
-// tail and the heads that follow it.
+// tail and the heads that follow it.  Bound by the memory: 1.18M x 512 fp32 rows are read at 6.1 TB/s, 0.94
+// of the measured copy rate; with dropout by the generator's integer work.
 constexpr int COLUMNS = 8;       // per lane
 constexpr int ROWS_AHEAD = 4;    // rows loaded before the first is added
 
@@ -459,13 +463,11 @@ __device__ __forceinline__ void store_sum(T* p, const float* sum, float factor) 
 // Three blocks an SM (85 registers a thread) take 1.18M x 512 with dropout from 598 to 532 us; narrow vectors
 // would spill.
 template <typename G, typename T, int V, bool DROP, bool ACCUMULATE>
-__global__ void __launch_bounds__(THREADS, V == COLUMNS ? 3 : 0) chunk_sum_kernel(int64_t n, uint32_t vocab, int channels, int slab,
-                                                            int lanes_log2, int chunk,
-                                                            int slabs, const uint2* __restrict__ pairs,
-                                                            const G* __restrict__ grad, float factor,
-                                                            uint32_t last, Draw draw, T* __restrict__ table,
-                                                            float* __restrict__ heads, float* __restrict__ tails,
-                                                            int stride) {
+__global__ void __launch_bounds__(THREADS, V == COLUMNS ? 3 : 0)
+    chunk_sum_kernel(int64_t n, uint32_t vocab, int channels, int slab, int lanes_log2, int chunk, int slabs,
+                     const uint2* __restrict__ pairs, const G* __restrict__ grad, float factor, uint32_t last,
+                     Draw draw, T* __restrict__ table, float* __restrict__ heads, float* __restrict__ tails,
+                     int stride) {
     constexpr int STEPS = COLUMNS / V;
     if (DROP) draw = resolve(draw);
     const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1);
@@ -686,7 +688,8 @@ __global__ void __launch_bounds__(THREADS) join_kernel(int64_t n, uint32_t vocab
 // the rows whose codeword is its own, groups them by codeword in shared memory (the scatter's ranking:
 // row order stays), adds each codeword's rows and writes every row of its range, zeros included.  Each
 // block reads all the ids, which is cheap while there are few; in return nothing waits for a second
-// launch.  A worker of 1 to FEW_LANES lanes (8 columns each) adds the rows of a codeword; one with many rows
+// launch: 4096 x 32 rows of 256 codewords take 18 us (events around the call), 27 with the sort, and at 8192
+// rows of 512 channels the sort is faster (35 us, 57 like this).  A worker of 1 to FEW_LANES lanes (8 columns each) adds the rows of a codeword; one with many rows
 // is added by the whole block, every worker a run of interleaved rows, and a tree.
 constexpr int FEW_THREADS = 512;
 constexpr int FEW_ROUNDS = 8;                        // ids per thread

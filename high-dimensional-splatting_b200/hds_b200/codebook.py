@@ -59,7 +59,11 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, pad
     others up, in the same pass.  The mask follows from (seed, offset) -- a step counter, say, as the
     offset -- and is drawn anew in the backward, never stored.  draw: an int64 tensor [2] = (seed, offset)
     on the device, used instead of the two numbers and read when the kernels run, so that a captured
-    graph can advance it; it must not change between a forward and its backward."""
+    graph can advance it; it must not change between a forward and its backward.
+
+    To capture a backward pass into a CUDA graph, keep no eager autograd graph of the same table alive
+    (torch ties the leaf's gradient to the stream of the first one); gaussian_rasterizer.embedding_backward
+    has no such rule."""
     table = table.contiguous()
     ids = ids.contiguous()
     if table.requires_grad and torch.is_grad_enabled():

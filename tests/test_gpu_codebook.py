@@ -68,7 +68,8 @@ SHAPES = [  # n, vocab, channels, spread
     (1000, 3, 64, 1), (1025, 255, 16, 4), (2048, 256, 40, 1), (4097, 257, 7, 2), (4096, 2048, 128, 1),
     (5000, 2047, 256, 3), (6000, 1, 264, 1), (3001, 70_000, 512, 1), (10_007, 65_535, 32, 1), (9000, 65_536, 24, 2),
     (20_011, 11, 5, 1), (12_345, 4_200_000, 2, 1), (40_000, 900, 72, 0), (900, 17, 1000, 1), (700, 50, 521, 1),
-    (100_000, 6, 32, 1), (131_072, 4096, 8, 4),
+    (100_000, 6, 32, 1), (131_072, 4096, 8, 4), (1_000_003, 3000, 8, 2), (990_000, 1500, 5, 0), (9, 4, 32_768, 1),
+    (11, 4, 20_001, 1), (6000, 3, 3000, 1), (4096, 32_768, 9, 1), (4097, 32_769, 16, 1),
 ]
 
 
@@ -156,6 +157,17 @@ def test_every_row_masked():
     out = hds_b200.embedding(table, ids, padding_id=-1)
     assert not out.detach().any()
     got, = torch.autograd.grad(out, table, torch.full_like(out, float("inf")))
+    assert not got.any()
+
+
+@pytest.mark.parametrize("n, c", [(100, 24), (6000, 24), (100, 13), (6000, 13)])
+def test_everything_dropped(n, c):
+    import hds_b200
+
+    table = torch.full((40, c), float("nan"), device="cuda", requires_grad=True)
+    out = hds_b200.embedding(table, torch.arange(n, device="cuda") % 40, dropout_p=1.0, seed=1)
+    assert not out.detach().any()
+    got, = torch.autograd.grad(out, table, torch.full_like(out, float("nan")))
     assert not got.any()
 
 
@@ -433,6 +445,38 @@ def test_captured_graphs_take_the_draw_of_each_replay():
         for i, (_, outs) in enumerate(graphs):
             want = step(i, offset=offset)
             assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+def test_a_large_gradient_captured_beside_eager_calls():
+    """The sort's blocks of more shared memory than the default, in a capture; eager gradients of the same
+    table before it and between the replays, and the kernels without autograd captured while an eager graph
+    of the table is alive."""
+    import hds_b200
+    from hds_b200 import gaussian_rasterizer as ext
+
+    rng = np.random.default_rng(9)
+    n, vocab, c = 1_100_000, 1500, 8
+    table = make_values(rng, (vocab, c), torch.float32).requires_grad_(True)
+    ids, grad = make_ids(rng, n, vocab, 2), make_values(rng, (n, c), torch.float32)
+
+    def step():
+        return torch.autograd.grad(hds_b200.embedding(table, ids), table, grad)[0]
+
+    want = step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(2):
+        got.zero_()
+        graph.replay()
+        assert torch.equal(got, want) and torch.equal(step(), want)
+    eager = hds_b200.embedding(table, ids)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ext.embedding_backward(grad, ids, vocab)
+    graph.replay()
+    assert torch.equal(got, want)
+    assert torch.equal(torch.autograd.grad(eager, table, grad)[0], want)
 
 
 def test_a_draw_that_moved_between_the_directions_is_refused():

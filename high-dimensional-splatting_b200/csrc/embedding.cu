@@ -688,8 +688,9 @@ __global__ void __launch_bounds__(THREADS) join_kernel(int64_t n, uint32_t vocab
 // the rows whose codeword is its own, groups them by codeword in shared memory (the scatter's ranking:
 // row order stays), adds each codeword's rows and writes every row of its range, zeros included.  Each
 // block reads all the ids, which is cheap while there are few; in return nothing waits for a second
-// launch: 4096 x 32 rows of 256 codewords take 18 us (events around the call), 27 with the sort, and at 8192
-// rows of 512 channels the sort is faster (35 us, 57 like this).  A worker of 1 to FEW_LANES lanes (8 columns each) adds the rows of a codeword; one with many rows
+// launch.  Measured with events around the call: 4096 x 32 rows of 256 codewords 18 us, 29 with the sort; 300 x 64
+// of 1000 12 and 28; 4096 x 512 of 256 37 and 31, where the six launches saved on the host still count; at
+// 8192 x 512 57 and 35.  A worker of 1 to FEW_LANES lanes (8 columns each) adds the rows of a codeword; one with many rows
 // is added by the whole block, every worker a run of interleaved rows, and a tree.
 constexpr int FEW_THREADS = 512;
 constexpr int FEW_ROUNDS = 8;                        // ids per thread

@@ -912,10 +912,11 @@ struct BackwardPlan {
         scan = !(tiles <= FEW_TILES || (tiles <= SOME_TILES && digit_bits <= SOME_DIGIT_BITS));
         // Long chunks write few partial sums (two rows of a chunk at most); but the chunks have to fill the
         // machine.  75,000 lanes with four rows of 32 bytes each in flight are about 10 MB, more than the
-        // memory's latency times its rate.
+        // memory's latency times its rate.  1.18M x 128 of 4096 popular codewords, 128 / 256 / 512 rows at most:
+        // 195, 182 and 185 us; 1.18M x 512 of 8192: 472, 456 and 499.
         const int64_t wanted = (int64_t)nn * std::max(channels, 1) / COLUMNS / 75000;
         chunk = 8;
-        while (chunk < 128 && chunk < wanted) chunk *= 2;
+        while (chunk < 256 && chunk < wanted) chunk *= 2;
         chunks = ((int64_t)nn + chunk - 1) / chunk;
         stride = (channels + COLUMNS - 1) / COLUMNS * COLUMNS;
         const int slabs = std::max(1, (channels + 32 * COLUMNS - 1) / (32 * COLUMNS));

@@ -65,9 +65,10 @@ def table_gradient(grad, ids, vocab, scale=1.0, padding_id=None, p=0.0, seed=0, 
     """(dtable [V, C], bound [V, C]) in 64 bits.  bound: how far an fp32 sum in the library's order may be.
 
     A sum along which at most P additions follow one another is off by at most P u sum |g| (u = 2^-24).
-    The library adds at most 128 rows one after another, then at most m / (8 * 64) partial sums each in 64
-    interleaved runs, then those: P <= min(m, 256 + m / 512) for m rows.  The factor and the product round
-    once each, adding 2 u; 1.01 covers the terms of order u^2."""
+    The library adds at most L rows one after another, L = 8 to 256, then the m / L + 2 parts of m rows: up
+    to 65 of them one after another, more in 64 interleaved runs and a tree of 6 steps.  So
+    P <= L + max(65, m / (64 L) + 8) <= 328 + m / 512, and never more than m.  The factor and the product
+    round once each, adding 2 u; 1.01 covers the terms of order u^2."""
     grad, ids = np.asarray(grad, np.float64), np.asarray(ids, np.int64).reshape(-1)
     c = grad.shape[-1]
     grad = grad.reshape(-1, c)
@@ -81,5 +82,5 @@ def table_gradient(grad, ids, vocab, scale=1.0, padding_id=None, p=0.0, seed=0, 
     np.add.at(sums, ids[there], g[there])
     np.add.at(size, ids[there], np.abs(g[there]))
     f = scale * keep_share_factor(p)
-    path = np.minimum(rows, 256 + rows / 512)[:, None] + 2
+    path = np.minimum(rows, 328 + rows / 512)[:, None] + 2
     return sums * f, 1.01 * path * U * size * abs(f)

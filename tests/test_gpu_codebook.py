@@ -238,6 +238,29 @@ def test_adding_into_a_buffer(c, vocab, p):
     assert torch.equal(buffer[absent], before[absent])
 
 
+def test_several_backward_passes_of_one_graph_and_second_derivatives():
+    import hds_b200
+
+    rng = np.random.default_rng(10)
+    table = make_values(rng, (50, 32), torch.float32).requires_grad_(True)
+    ids = make_ids(rng, 400, 50)
+    out = hds_b200.dropout(hds_b200.embedding(table, ids), 0.5, seed=3)
+    grads = [make_values(rng, (400, 32), torch.float32) for _ in range(3)]
+    got = [torch.autograd.grad(out, table, g, retain_graph=True)[0] for g in grads]
+    kept = torch.from_numpy(plain.keep_mask(0, 400 * 32, 0.5, 3, 0).reshape(400, 32))
+    for g, w in zip(got, grads):
+        assert_gradient(g, torch.where(kept, 2 * w.cpu(), torch.zeros(())), ids, 50)
+    # A second derivative of dropout is dropout again; that of the lookup's gradient is refused.
+    x = make_values(rng, (64, 8), torch.float32).requires_grad_(True)
+    y = hds_b200.dropout(x, 0.5, seed=4)
+    w = make_values(rng, (64, 8), torch.float32).requires_grad_(True)
+    first, = torch.autograd.grad(y, x, w, create_graph=True)
+    second, = torch.autograd.grad(first.sum(), w)
+    assert torch.equal(second.cpu(), expected_dropout(torch.ones(64, 8), 0.5, 4, 0, False))
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        torch.autograd.grad(out, table, grads[0].clone().requires_grad_(True), create_graph=True)
+
+
 def test_gradient_is_added_into_the_leaf():
     import hds_b200
 

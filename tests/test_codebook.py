@@ -1,7 +1,5 @@
 """CPU checks of the codebook lookup and dropout: the plain implementation they are tested against, and
 the refusals that happen before any device work."""
-import ctypes
-
 import numpy as np
 import pytest
 
@@ -146,4 +144,3 @@ def test_python_refusals():
         with pytest.raises(ValueError, match=r"in \[0, 1\]"):
             hds_b200.dropout(table, p)
     assert hds_b200.dropout(table, 0.0) is table  # nothing to drop
-    assert ctypes.sizeof(ctypes.c_uint64) == 8

@@ -23,26 +23,32 @@ class Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, ids, dtype, how):
         """how: embedding()'s (scale, padding_id, dropout_p, seed, offset, draw)."""
+        scale, padding_id, dropout_p, seed, offset, draw = how
+        out = _ext.embedding(table, ids, dtype, *how)
         ctx.leaf = table if (rasterizer.ACCUMULATE_INTO_LEAF_GRAD and table.is_leaf) else None
-        ctx.table = (table.shape[0], table.dtype)
-        ctx.how = how
-        ctx.save_for_backward(ids, how[-1])
-        return _ext.embedding(table, ids, dtype, *how)
+        ctx.table = (table.shape, table.dtype)
+        # What the backward passes on, checked above: autograd runs it in a thread of its own, where the
+        # host's every step costs more than here.
+        ctx.how = (scale, padding_id, *_ext._draw(dropout_p, seed, offset, draw, table.device))
+        ctx.draw = draw  # alive: how has its address
+        ctx.save_for_backward(ids, draw)
+        return out
 
     @staticmethod
     def backward(ctx, grad):
         if grad.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("the gradient of embedding() cannot be differentiated again")
         ids, _ = ctx.saved_tensors  # raises if the ids or the draw have changed since
-        rows, dtype = ctx.table
+        shape, dtype = ctx.table
         grad = grad.contiguous()
         target = ctx.leaf.grad if ctx.leaf is not None else None
         if (target is not None and grad.dtype == torch.float32 and target.dtype == torch.float32
-                and target.is_contiguous() and target.shape == (rows, grad.shape[-1])
-                and target.device == grad.device):
-            _ext.embedding_backward_into(target, grad, ids, *ctx.how)
+                and target.is_contiguous() and target.shape == shape and target.device == grad.device):
+            _ext._sum_by_id(grad, ids, target, 1, *ctx.how)
             return None, None, None, None
-        return _ext.embedding_backward(grad, ids, rows, dtype, *ctx.how), None, None, None
+        grad_table = torch.empty(shape, dtype=dtype, device=grad.device)
+        _ext._sum_by_id(grad, ids, grad_table, 0, *ctx.how)
+        return grad_table, None, None, None
 
 
 def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, padding_id: int | None = None,

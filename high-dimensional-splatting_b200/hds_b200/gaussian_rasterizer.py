@@ -530,7 +530,13 @@ def _embedding_backward(grad, ids, grad_table, accumulate, scale, padding_id, dr
     if grad.device != dev or grad.shape != (*ids.shape, c):
         raise RuntimeError(f"grad must be {(*ids.shape, c)} on the table's device")
     _check_lookup(grad_table.dtype, grad.dtype, ids, dev, padding_id)
-    threshold, seed, offset, draw_ptr = _draw(dropout_p, seed, offset, draw, dev)
+    _sum_by_id(grad, ids, grad_table, accumulate, scale, padding_id, *_draw(dropout_p, seed, offset, draw, dev))
+
+
+def _sum_by_id(grad, ids, grad_table, accumulate, scale, padding_id, threshold, seed, offset, draw_ptr):
+    """_embedding_backward of arguments that have been checked (autograd's: those of the forward)."""
+    dev = grad_table.device
+    v, c = grad_table.shape
     n = ids.numel()
     need = lib.hds_embedding_backward_scratch_bytes(n, v, c)
     scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None

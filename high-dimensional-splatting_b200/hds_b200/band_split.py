@@ -51,7 +51,7 @@ def gather_rows(rows: torch.Tensor, ids: torch.Tensor) -> torch.Tensor:
     if rows.is_cuda:
         from .gaussian_rasterizer import embedding
 
-        return embedding(rows, ids)
+        return embedding(rows, ids.to(rows.device))
     return rows[ids].contiguous()
 
 
@@ -60,7 +60,7 @@ def add_rows(target: torch.Tensor, ids: torch.Tensor, rows: torch.Tensor) -> Non
     if target.is_cuda:
         from .gaussian_rasterizer import embedding_backward_into
 
-        embedding_backward_into(target, rows, ids)
+        embedding_backward_into(target, rows, ids.to(target.device))
     else:
         target.index_add_(0, ids, rows)
 

@@ -221,21 +221,25 @@ def test_unaligned_and_strided_inputs(c, dtype, p):
 
 @pytest.mark.parametrize("c, vocab", [(32, 500), (45, 500), (256, 20_000), (8, 3)])
 @pytest.mark.parametrize("p", [0.0, 0.2])
-def test_adding_into_a_buffer(c, vocab, p):
+@pytest.mark.parametrize("n, skip", [(2500, 0), (2500, 3), (7000, 0), (7000, 6)])
+def test_adding_into_a_buffer(c, vocab, p, n, skip):
+    """skip: where the table's gradient begins in a flat buffer of all parameters' gradients."""
     from hds_b200 import gaussian_rasterizer as ext
 
     rng = np.random.default_rng(vocab + c)
-    n = 2500
     ids = make_ids(rng, n, vocab, 3, padding=-1)
     grad = make_values(rng, (n, c), torch.float32)
     before = make_values(rng, (vocab, c), torch.float32)
-    buffer = before.clone()
+    flat = torch.zeros(vocab * c + 2 * skip, device="cuda")
+    buffer = flat[skip:skip + vocab * c].view(vocab, c)
+    buffer.copy_(before)
     how = dict(scale=0.5, padding_id=-1, seed=3, offset=8)
     ext.embedding_backward_into(buffer, grad, ids, dropout_p=p, **how)
     assert_gradient(buffer, grad, ids, vocab, p=p, before=before, **how)
     absent = torch.ones(vocab, dtype=torch.bool, device="cuda")
     absent[ids[ids >= 0]] = False
     assert torch.equal(buffer[absent], before[absent])
+    assert not flat[:skip].any() and not flat[skip + vocab * c:].any()
 
 
 def test_several_backward_passes_of_one_graph_and_second_derivatives():
@@ -349,7 +353,7 @@ def expected_dropout(x, p, seed, offset, rows):
 
 @pytest.mark.parametrize("dtype", list(TYPES.values()), ids=list(TYPES))
 @pytest.mark.parametrize("shape", [(1,), (7,), (8,), (3, 5), (256, 32), (255, 33), (1000, 75), (17, 4096), (4097, 2),
-                                   (5, 6, 9), (100_003, 1), (1, 70_001), (2, 3, 16)])
+                                   (5, 6, 9), (100_003, 1), (1, 70_001), (2, 3, 16), (5, 40_000), (7, 33_003)])
 @pytest.mark.parametrize("rows", [False, True], ids=["elements", "rows"])
 @pytest.mark.parametrize("p", [0.1, 0.75])
 def test_dropout_and_its_gradient(shape, dtype, rows, p):

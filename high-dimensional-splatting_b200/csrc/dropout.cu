@@ -106,7 +106,8 @@ __global__ void __launch_bounds__(DROPOUT_THREADS) dropout_rows_kernel(int64_t n
     for (int t = 0; t < TILES; t++) {
         if (t == 0 || row_width < 8) {
             const int64_t group0 = (row0 + rows_on(t * TILE_ELEMENTS)) >> 3;
-            bits = philox4x32_10((uint32_t)(group0 + lane), (uint32_t)((uint64_t)(group0 + lane) >> 32), draw).bits(last);
+            const uint64_t group = (uint64_t)(group0 + lane);
+            bits = philox4x32_10((uint32_t)group, (uint32_t)(group >> 32), draw).bits(last);
             first = (int)(row0 - 8 * group0);
         }
         const auto row_kept = [&](uint32_t on) -> uint32_t {  // the row `on` rows from row0

@@ -488,7 +488,8 @@ __global__ void __launch_bounds__(THREADS, V == COLUMNS ? 3 : 0)
     const auto put = [&](float* partial) {
 #pragma unroll
         for (int k = 0; k < STEPS; k++)
-            if (column(k) < width) store_sum<float, V, false>(partial + id * stride + c0 + column(k), sum + k * V, 1.0f);
+            if (column(k) < width)
+                store_sum<float, V, false>(partial + id * stride + c0 + column(k), sum + k * V, 1.0f);
     };
     const auto finish = [&]() {  // the current codeword ends here
         if (began_earlier) {
@@ -690,8 +691,8 @@ __global__ void __launch_bounds__(THREADS) join_kernel(int64_t n, uint32_t vocab
 // block reads all the ids, which is cheap while there are few; in return nothing waits for a second
 // launch.  Measured with events around the call: 4096 x 32 rows of 256 codewords 18 us, 29 with the sort; 300 x 64
 // of 1000 12 and 28; 4096 x 512 of 256 37 and 31, where the six launches saved on the host still count; at
-// 8192 x 512 57 and 35.  A worker of 1 to FEW_LANES lanes (8 columns each) adds the rows of a codeword; one with many rows
-// is added by the whole block, every worker a run of interleaved rows, and a tree.
+// 8192 x 512 57 and 35.  A worker of 1 to FEW_LANES lanes (8 columns each) adds the rows of a codeword; one
+// with many rows is added by the whole block, every worker a run of interleaved rows, and a tree.
 constexpr int FEW_THREADS = 512;
 constexpr int FEW_ROUNDS = 8;                        // ids per thread
 constexpr int FEW_ROWS = FEW_THREADS * FEW_ROUNDS;  // 4096
@@ -828,8 +829,8 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(int n, int channe
 #pragma unroll
         for (int k = 0; k < STEPS; k++)
             if (column(k) < width)
-                store_sum<T, V, ACCUMULATE>(table + (int64_t)(first + codeword) * channels + c0 + column(k), sum + k * V,
-                                            factor);
+                store_sum<T, V, ACCUMULATE>(table + (int64_t)(first + codeword) * channels + c0 + column(k),
+                                            sum + k * V, factor);
     };
     for (int v = worker; v < here; v += workers) {
         const uint32_t from = s_start[v], to = s_start[v + 1];
@@ -1117,8 +1118,9 @@ extern "C" int hds_embedding_backward(int64_t n, int64_t vocab, int64_t columns,
                 return HDS_OK;
             };
             // Whole vectors or single elements: at these sizes the widths between would save nothing.
-            if (v == COLUMNS) return launch(few_rows_kernel<G, T, COLUMNS, decltype(drop)::value, decltype(add)::value>);
-            return launch(few_rows_kernel<G, T, 1, decltype(drop)::value, decltype(add)::value>);
+            constexpr bool DROP = decltype(drop)::value, ADD = decltype(add)::value;
+            if (v == COLUMNS) return launch(few_rows_kernel<G, T, COLUMNS, DROP, ADD>);
+            return launch(few_rows_kernel<G, T, 1, DROP, ADD>);
         });
     }
     // The sums write only the rows of codewords that occur.
@@ -1149,8 +1151,8 @@ extern "C" int hds_embedding_backward(int64_t n, int64_t vocab, int64_t columns,
                     digits, tiles, counts, totals);
                 HDS_CHECK_LAUNCH("scan_kernel");
             }
-            scatter<<<tiles, SORT_THREADS, shared, stream>>>((int)n, source, shift, plan.digit_bits, tiles, plan.scan, counts,
-                                                             totals, pairs);
+            scatter<<<tiles, SORT_THREADS, shared, stream>>>((int)n, source, shift, plan.digit_bits, tiles, plan.scan,
+                                                             counts, totals, pairs);
             HDS_CHECK_LAUNCH("scatter_kernel");
             return HDS_OK;
         };
@@ -1173,9 +1175,9 @@ extern "C" int hds_embedding_backward(int64_t n, int64_t vocab, int64_t columns,
         if (int rc = with_vector(v, [&](auto width) -> int {
                 chunk_sum_kernel<G, T, decltype(width)::value, decltype(drop)::value, decltype(add)::value>
                     <<<sum_grid, THREADS, 0, stream>>>(n, (uint32_t)vocab, channels, plan.slab, plan.lanes_log2,
-                                                       plan.chunk, slabs, sorted,
-                                                       static_cast<const G*>(grad), factor,
-                                                       below_last(drop_threshold), d, static_cast<T*>(grad_table), heads, tails, plan.stride);
+                                                       plan.chunk, slabs, sorted, static_cast<const G*>(grad), factor,
+                                                       below_last(drop_threshold), d, static_cast<T*>(grad_table),
+                                                       heads, tails, plan.stride);
                 HDS_CHECK_LAUNCH("chunk_sum_kernel");
                 return HDS_OK;
             }))

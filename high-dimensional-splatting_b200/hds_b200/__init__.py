@@ -16,5 +16,6 @@ from .rasterizer import FEATURE_SLICE_WIDTH, RasterizeGaussians, _get_rasterizer
 from .sh import view_colors
 
 __all__ = ["rasterize", "project_gaussians", "project_gaussians_raw", "view_colors", "embedding", "dropout",
-           "accumulate_leaf_grads", "Embedding", "Dropout", "RasterizeGaussians", "ProjectGaussians", "ProjectGaussiansRaw", "quat_to_rotmat", "_get_rasterizer",
-           "FEATURE_SLICE_WIDTH", "NEAR_PLANE", "LOW_PASS", "JACOBIAN_FOV_SCALE"]
+           "accumulate_leaf_grads", "Embedding", "Dropout", "RasterizeGaussians", "ProjectGaussians",
+           "ProjectGaussiansRaw", "quat_to_rotmat", "_get_rasterizer", "FEATURE_SLICE_WIDTH",
+           "NEAR_PLANE", "LOW_PASS", "JACOBIAN_FOV_SCALE"]

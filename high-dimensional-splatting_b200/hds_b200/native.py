@@ -151,8 +151,15 @@ def on_device(device):
 
 
 def device_status(device=None) -> int:
-    """Reads and clears the device-side failure word (0 = no bounded wait ran out and no codebook id lay
-    outside its table)."""
+    """Reads and clears the failure word of a device (None, or a device without an index: the current one).
+    0 = no bounded wait ran out and no codebook id lay outside its table.  Every device has a word of its
+    own, which the library finds through the current device, so that device is made current."""
+    import torch
+
+    device = torch.device("cuda" if device is None else device)
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
     out = c_int(0)
-    check(lib.hds_device_status(ctypes.byref(out), stream_of(device)))
+    with on_device(device):
+        check(lib.hds_device_status(ctypes.byref(out), stream_of(device)))
     return out.value

@@ -1,0 +1,41 @@
+"""The codebook operators on the GPU, called in ways that are allowed and rare."""
+import subprocess
+import sys
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def test_the_status_may_be_the_first_call_of_a_program():
+    code = ("import sys; sys.path.insert(0, 'high-dimensional-splatting_b200'); from hds_b200 import native; "
+            "print(native.device_status({}), native.device_status())")
+    for device in ("", "'cuda:0'", "0"):
+        done = subprocess.run([sys.executable, "-c", code.format(device)], capture_output=True, text=True, timeout=240)
+        assert done.returncode == 0 and done.stdout.split() == ["0", "0"], done.stderr
+
+
+def test_on_a_device_that_is_not_the_current_one():
+    """Values, gradient, dropout and the status word of the tensors' own device."""
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two devices")
+    import hds_b200
+    from hds_b200 import native
+
+    torch.cuda.set_device(0)
+    gen = torch.Generator().manual_seed(1)
+    table = torch.randn(40, 24, generator=gen)
+    grad = torch.randn(6000, 24, generator=gen)
+    for ids in (torch.arange(6000) % 40, torch.arange(6000) % 41):
+        got = []
+        for device in ("cuda:0", "cuda:1"):
+            leaf = table.to(device).requires_grad_(True)
+            out = hds_b200.dropout(hds_b200.embedding(leaf, ids.to(device), dropout_p=0.2, seed=1), 0.3, seed=2)
+            got.append((out.detach().cpu(), torch.autograd.grad(out, leaf, grad.to(device))[0].cpu()))
+            torch.cuda.synchronize(device)
+            other = "cuda:0" if device == "cuda:1" else "cuda:1"
+            assert native.device_status(other) == 0
+            assert native.device_status(device) == int(ids.max() == 40)
+        assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    assert torch.cuda.current_device() == 0

@@ -832,9 +832,18 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(int n, int channe
                 store_sum<T, V, ACCUMULATE>(table + (int64_t)(first + codeword) * channels + c0 + column(k),
                                             sum + k * V, factor);
     };
+    const auto clear = [&](int codeword) {  // +0, as the memset of the sorted form leaves it
+#pragma unroll
+        for (int k = 0; k < STEPS; k++)
+            if (column(k) < width)
+                store<T, V>(table + (int64_t)(first + codeword) * channels + c0 + column(k), Vec<T, V>{});
+    };
     for (int v = worker; v < here; v += workers) {
         const uint32_t from = s_start[v], to = s_start[v + 1];
-        if (ACCUMULATE && from == to) continue;
+        if (from == to) {
+            if (!ACCUMULATE) clear(v);
+            continue;
+        }
         if (to - from > SHORT_ROWS) {
             if (lane == 0) s_long_codeword[atomicAdd(&s_long, 1)] = (uint16_t)v;
             continue;
@@ -951,9 +960,12 @@ int check_arguments(const char* what, int64_t n, int64_t vocab, int64_t channels
                 HDS_ERR_UNSUPPORTED, "%s: values must be of the table's type or fp32", what);
     HDS_REQUIRE(ids_type == HDS_TYPE_I32 || ids_type == HDS_TYPE_I64, HDS_ERR_UNSUPPORTED,
                 "%s: ids must be int32 or int64", what);
-    HDS_REQUIRE(scale - scale == 0.0, HDS_ERR_INVALID, "%s: scale must be finite", what);
     HDS_REQUIRE(drop_threshold >= 0 && drop_threshold <= DROP_ONE, HDS_ERR_INVALID,
                 "%s: dropout threshold %d outside 0 to 65536", what, drop_threshold);
+    // The kernels multiply by the fp32 factor: infinite, it would make NaN of every zero.
+    const float factor = keep_factor(scale, drop_threshold);
+    HDS_REQUIRE(scale - scale == 0.0 && factor - factor == 0.0f, HDS_ERR_INVALID,
+                "%s: scale must be finite, and in fp32 by the kept share's reciprocal too", what);
     // The kernels keep the generator's upper group word out of the lanes: it is 0.
     HDS_REQUIRE(drop_threshold == 0 || n * channels <= HDS_EMBEDDING_MAX_DROPOUT, HDS_ERR_TOO_LARGE,
                 "%s: dropout of %lld values (2^35 at most)", what, (long long)(n * channels));

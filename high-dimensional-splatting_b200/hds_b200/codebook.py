@@ -57,6 +57,7 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, pad
     """scale * table[ids]: the features [*ids.shape, C] of the codeword ids under the codebook table
     [V, C] (float32, bfloat16 or float16; ids int32 or int64), in `dtype` (the table's type, or float32:
     the type rasterize takes).  Differentiable in table; the same backward call gives the same bits.
+    scale, times the reciprocal of the kept share, must be finite in float32.
 
     padding_id: ids with this value (a negative one, say, for gaussians without a codeword) give rows of
     zeros and no gradient.  Any other id outside [0, V) does too, and sets native.device_status().

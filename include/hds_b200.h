@@ -320,7 +320,8 @@ int hds_densify_apply(int n_old, int n_new, int segments, const int* widths, int
  * memory (8-byte aligned), read when the kernels run instead of the two arguments, so that a captured
  * graph can take a new mask at every replay.  Dropped elements are 0 whatever the input holds.
  *
- * hds_embedding_forward: out[i] = scale * table[ids[i]] [n, channels].  An id equal to padding_id (when
+ * hds_embedding_forward: out[i] = scale * table[ids[i]] [n, channels]; scale * 65536 / (65536 - T) must be
+ * finite in fp32, in both directions.  An id equal to padding_id (when
  * has_padding) gives a row of zeros and takes no gradient.  So does any other id outside [0, vocab),
  * which also records HDS_ERR_INVALID in the device status (hds_device_status).
  *

@@ -61,3 +61,33 @@ def test_the_status_is_read_on_its_own_device(monkeypatch, device, index):
     assert native.device_status(device) == index + 1
     assert devices.seen == [(index, 100 + index)]
     assert devices.current == 0
+
+
+F32, BF16, F16, I32, I64 = range(5)
+HALF = 32768  # a dropout threshold of 0.5
+
+
+@pytest.mark.parametrize("scale, threshold", [(1e39, 0), (-1e39, 0), (3.5e38, 0), (3e38, HALF), (-3e38, HALF), (1e38, 65535),
+                                              (float("inf"), 0), (float("nan"), 0), (float("inf"), 65536)])
+def test_scales_that_are_infinite_in_fp32_are_refused(scale, threshold):
+    """The factor scale * 65536 / (65536 - T) is used in fp32; infinite, it would turn zeros into NaN."""
+    from hds_b200 import native
+
+    lib = native.lib
+    for call in (lambda: lib.hds_embedding_forward(4, 4, 8, F32, 256, I64, 256, 0, 0, scale, threshold, 0, 0, None, F32,
+                                                   256, None),
+                 lambda: lib.hds_embedding_backward(100_000, 4, 8, F32, 256, I64, 256, 0, 0, scale, threshold, 0, 0, None,
+                                                    F32, 256, 0, 256, 1 << 30, None)):
+        assert call() == 1
+        assert "finite" in lib.hds_last_error().decode()
+
+
+@pytest.mark.parametrize("scale, threshold", [(3.4e38, 0), (-3.4e38, 0), (1.7e38, HALF), (1e39, 65536), (0.0, 0)])
+def test_scales_that_fit_fp32_are_taken(scale, threshold):
+    """The largest factors that fit (with nothing to look up), and any finite scale of nothing kept."""
+    from hds_b200 import native
+
+    lib = native.lib
+    assert lib.hds_embedding_forward(0, 4, 8, F32, None, I64, None, 0, 0, scale, threshold, 0, 0, None, F32, None, None) == 0
+    assert lib.hds_embedding_backward(0, 0, 8, F32, None, I64, None, 0, 0, scale, threshold, 0, 0, None, F32, None, 0, None,
+                                      0, None) == 0

@@ -1,6 +1,7 @@
 """The codebook operators on the GPU, called in ways that are allowed and rare."""
 import subprocess
 import sys
+from pathlib import Path
 
 import pytest
 
@@ -12,7 +13,8 @@ def test_the_status_may_be_the_first_call_of_a_program():
     code = ("import sys; sys.path.insert(0, 'high-dimensional-splatting_b200'); from hds_b200 import native; "
             "print(native.device_status({}), native.device_status())")
     for device in ("", "'cuda:0'", "0"):
-        done = subprocess.run([sys.executable, "-c", code.format(device)], capture_output=True, text=True, timeout=240)
+        done = subprocess.run([sys.executable, "-c", code.format(device)], capture_output=True, text=True, timeout=240,
+                              cwd=Path(__file__).resolve().parent.parent)
         assert done.returncode == 0 and done.stdout.split() == ["0", "0"], done.stderr
 
 
@@ -39,3 +41,16 @@ def test_on_a_device_that_is_not_the_current_one():
             assert native.device_status(device) == int(ids.max() == 40)
         assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
     assert torch.cuda.current_device() == 0
+
+
+@pytest.mark.parametrize("n", [100, 6000])  # one launch, and the sorted form
+@pytest.mark.parametrize("c", [24, 13])
+@pytest.mark.parametrize("scale", [-2.0, 3e38])
+def test_rows_of_absent_codewords_are_plain_zeros(n, c, scale):
+    from hds_b200 import gaussian_rasterizer as ext
+
+    ids = torch.arange(n, device="cuda") % 20
+    got = ext.embedding_backward(torch.randn(n, c, device="cuda"), ids, 50, scale=scale)
+    absent = got[20:].cpu()
+    assert torch.equal(absent, torch.zeros(30, c)) and not torch.signbit(absent).any()
+    assert got[:20].any()

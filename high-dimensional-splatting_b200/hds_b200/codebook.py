@@ -36,7 +36,7 @@ class Embedding(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad):
-        if grad.requires_grad and torch.is_grad_enabled():
+        if (grad.requires_grad and torch.is_grad_enabled()) or rasterizer.has_tangent(grad):
             raise RuntimeError("the gradient of embedding() cannot be differentiated again")
         ids, _ = ctx.saved_tensors  # raises if the ids or the draw have changed since
         shape, dtype = ctx.table
@@ -73,6 +73,6 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, pad
     has no such rule."""
     table = table.contiguous()
     ids = ids.contiguous()
-    if table.requires_grad and torch.is_grad_enabled():
+    if rasterizer.needs_node(table):
         return Embedding.apply(table, ids, dtype, (scale, padding_id, dropout_p, seed, offset, draw))
     return _ext.embedding(table, ids, dtype, scale, padding_id, dropout_p, seed, offset, draw)

@@ -5,6 +5,7 @@ from __future__ import annotations
 import torch
 
 from . import gaussian_rasterizer as _ext
+from . import rasterizer
 
 
 class Dropout(torch.autograd.Function):
@@ -38,6 +39,6 @@ def dropout(x: torch.Tensor, p: float, *, seed: int = 0, offset: int = 0, rows: 
     if _ext.drop_threshold(p) == 0:
         return x
     x = x.contiguous()
-    if x.requires_grad and torch.is_grad_enabled():
+    if rasterizer.needs_node(x):
         return Dropout.apply(x, (p, seed, offset, rows, draw))
     return _ext.dropout(x, p, seed, offset, rows, draw)

@@ -53,6 +53,18 @@ class accumulate_leaf_grads:
         return False
 
 
+def has_tangent(t: torch.Tensor) -> bool:
+    """Whether t carries a forward-mode tangent (torch.autograd.forward_ad)."""
+    return torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+
+
+def needs_node(t: torch.Tensor) -> bool:
+    """Whether a call on t has to go through its autograd node: for t's gradient, for a tangent (the node
+    refuses what the kernels would lose) and for torch.jit.trace (which records the node, but not what a
+    kernel writes through a pointer).  Other calls save the node's 5 us on the host."""
+    return (t.requires_grad and torch.is_grad_enabled()) or has_tangent(t) or torch.jit.is_tracing()
+
+
 def _get_rasterizer() -> ModuleType:
     """The extension module with the reference's ten entry points (see gaussian_rasterizer.py)."""
     return _ext

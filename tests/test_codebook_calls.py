@@ -1,7 +1,9 @@
 """CPU checks of the host side of the codebook operators: which device, stream and tensors a call hands to
 the library, with a fake in the library's place, and what it does not hand over."""
 import contextlib
+import ctypes
 
+import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -91,3 +93,99 @@ def test_scales_that_fit_fp32_are_taken(scale, threshold):
     assert lib.hds_embedding_forward(0, 4, 8, F32, None, I64, None, 0, 0, scale, threshold, 0, 0, None, F32, None, None) == 0
     assert lib.hds_embedding_backward(0, 0, 8, F32, None, I64, None, 0, 0, scale, threshold, 0, 0, None, F32, None, 0, None,
                                       0, None) == 0
+
+
+class CpuKernels:
+    """The extension module's two operators and the gradient on CPU tensors, written through the
+    tensors' addresses as the kernels do: torch does not see what they compute.  Dropout keeps all."""
+
+    def __init__(self, monkeypatch):
+        from hds_b200 import gaussian_rasterizer as ext
+
+        monkeypatch.setattr(ext, "_check", lambda t, name: None)
+        monkeypatch.setattr(ext, "on_device", lambda device: contextlib.nullcontext())
+        monkeypatch.setattr(ext, "stream_of", lambda device: 0)
+        monkeypatch.setattr(ext, "lib", self)
+        self.calls = []
+
+    @staticmethod
+    def at(address, count, kind=ctypes.c_float):
+        return np.ctypeslib.as_array((kind * count).from_address(address))
+
+    def hds_embedding_forward(self, n, vocab, c, table_type, table, ids_type, ids, has_padding, padding_id, scale,
+                              threshold, seed, offset, draw, out_type, out, stream):
+        self.calls.append(("forward", draw and list(self.at(draw, 2, ctypes.c_int64))))
+        rows = self.at(table, vocab * c).reshape(vocab, c)[self.at(ids, n, ctypes.c_int64)]
+        self.at(out, n * c)[:] = np.float32(scale) * rows.reshape(-1)
+        return 0
+
+    def hds_embedding_backward_scratch_bytes(self, n, vocab, c):
+        return 0
+
+    def hds_embedding_backward(self, n, vocab, c, grad_type, grad, ids_type, ids, has_padding, padding_id, scale,
+                               threshold, seed, offset, draw, table_type, grad_table, accumulate, scratch, bytes_, stream):
+        self.calls.append(("backward", draw and list(self.at(draw, 2, ctypes.c_int64))))
+        out = self.at(grad_table, vocab * c).reshape(vocab, c)
+        if not accumulate:
+            out[:] = 0
+        np.add.at(out, self.at(ids, n, ctypes.c_int64), np.float32(scale) * self.at(grad, n * c).reshape(n, c))
+        return 0
+
+    def hds_dropout(self, rows, c, type_, x, threshold, whole_rows, seed, offset, draw, y, stream):
+        self.calls.append(("dropout", draw and list(self.at(draw, 2, ctypes.c_int64))))
+        self.at(y, rows * c)[:] = self.at(x, rows * c)
+        return 0
+
+
+def small_lookup(**more):
+    table = torch.arange(12.0).reshape(4, 3)
+    return table, torch.tensor([2, 0, 2]), dict(scale=2.0, seed=1, offset=2, **more)
+
+
+def test_forward_mode_is_refused_and_not_lost(monkeypatch):
+    """A tangent has requires_grad == False.  The operators have no forward mode; a call that goes past the
+    autograd node would return a constant."""
+    import hds_b200
+    from torch.autograd import forward_ad
+
+    kernels = CpuKernels(monkeypatch)
+    table, ids, how = small_lookup()
+    assert torch.equal(hds_b200.embedding(table, ids, **how), 2 * table[ids])
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(table, torch.ones_like(table))
+        for call in (lambda: hds_b200.embedding(dual, ids, **how), lambda: hds_b200.dropout(dual, 0.5, seed=1)):
+            with pytest.raises(NotImplementedError, match="jvp"):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="jvp"):
+                call()
+        # The backward passes are maps of their own; so is a tangent of what goes into them.
+        leaf = table.clone().requires_grad_(True)
+        grad = forward_ad.make_dual(torch.ones(3, 3), torch.ones(3, 3))
+        out = hds_b200.embedding(leaf, ids, **how)
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            torch.autograd.grad(out, leaf, grad)
+        out = hds_b200.dropout(leaf, 0.5, seed=1)
+        with pytest.raises(NotImplementedError, match="jvp"):
+            torch.autograd.grad(out, leaf, forward_ad.make_dual(torch.ones(4, 3), torch.ones(4, 3)))
+        # Inside a level, tensors without a tangent go through as ever.
+        assert torch.equal(hds_b200.embedding(table, ids, **how), 2 * table[ids])
+    assert [c[0] for c in kernels.calls].count("backward") == 0
+
+
+def test_traced_calls_run_the_kernels(monkeypatch):
+    """torch.jit.trace records torch's operators; the kernels' writes are none, so the node is recorded."""
+    import hds_b200
+
+    CpuKernels(monkeypatch)
+    table, ids, how = small_lookup()
+
+    def lookup(t):
+        return hds_b200.embedding(t, ids, **how)
+
+    def drop(t):
+        return hds_b200.dropout(t, 0.5, seed=1)
+
+    for f, want in ((lookup, lambda t: 2 * t[ids]), (drop, lambda t: t)):
+        traced = torch.jit.trace(f, (table,), check_trace=False)
+        for t in (table, table + 1, -table):
+            assert torch.equal(traced(t), want(t))

@@ -54,3 +54,20 @@ def test_rows_of_absent_codewords_are_plain_zeros(n, c, scale):
     absent = got[20:].cpu()
     assert torch.equal(absent, torch.zeros(30, c)) and not torch.signbit(absent).any()
     assert got[:20].any()
+
+
+def test_forward_mode_is_refused_and_traces_run_the_kernels():
+    import hds_b200
+    from torch.autograd import forward_ad
+
+    table, ids = torch.randn(9, 16, device="cuda"), torch.arange(40, device="cuda") % 9
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(table, torch.ones_like(table))
+        with pytest.raises(NotImplementedError, match="jvp"):
+            hds_b200.embedding(dual, ids)
+        with pytest.raises(NotImplementedError, match="jvp"):
+            hds_b200.dropout(dual, 0.5, seed=1)
+    traced = torch.jit.trace(lambda t: hds_b200.embedding(t, ids), (table,), check_trace=False)
+    assert torch.equal(traced(table + 1), (table + 1)[ids])
+    traced = torch.jit.trace(lambda t: hds_b200.dropout(t, 0.5, seed=1), (table,), check_trace=False)
+    assert torch.equal(traced(table + 1), hds_b200.dropout(table + 1, 0.5, seed=1))

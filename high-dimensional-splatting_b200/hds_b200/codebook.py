@@ -27,27 +27,32 @@ class Embedding(torch.autograd.Function):
         out = _ext.embedding(table, ids, dtype, *how)
         ctx.leaf = table if (rasterizer.ACCUMULATE_INTO_LEAF_GRAD and table.is_leaf) else None
         ctx.table = (table.shape, table.dtype)
-        # What the backward passes on, checked above: autograd runs it in a thread of its own, where the
-        # host's every step costs more than here.
-        ctx.how = (scale, padding_id, *_ext._draw(dropout_p, seed, offset, draw, table.device))
-        ctx.draw = draw  # alive: how has its address
-        ctx.save_for_backward(ids, draw)
+        # The backward's numbers, checked above.
+        threshold, seed, offset, _ = _ext._draw(dropout_p, seed, offset, draw, table.device)
+        ctx.how = (scale, padding_id, threshold, seed, offset)
+        ctx.save_for_backward(ids, draw if threshold else None)
         return out
 
     @staticmethod
     def backward(ctx, grad):
         if (grad.requires_grad and torch.is_grad_enabled()) or rasterizer.has_tangent(grad):
             raise RuntimeError("the gradient of embedding() cannot be differentiated again")
-        ids, _ = ctx.saved_tensors  # raises if the ids or the draw have changed since
+        ids, draw = ctx.saved_tensors  # raises if the ids or the draw have changed since
         shape, dtype = ctx.table
         grad = grad.contiguous()
+        # What hooks on saved tensors or an assignment to .data have put in their place goes to a kernel as
+        # an address.
+        _ext._check_ids(ids, grad.device)
+        if ids.shape != grad.shape[:-1]:
+            raise RuntimeError(f"ids were {tuple(grad.shape[:-1])} in the forward, and are {tuple(ids.shape)} now")
+        how = (*ctx.how, _ext._draw_address(draw, grad.device))
         target = ctx.leaf.grad if ctx.leaf is not None else None
         if (target is not None and grad.dtype == torch.float32 and target.dtype == torch.float32
                 and target.is_contiguous() and target.shape == shape and target.device == grad.device):
-            _ext._sum_by_id(grad, ids, target, 1, *ctx.how)
+            _ext._sum_by_id(grad, ids, target, 1, *how)
             return None, None, None, None
         grad_table = torch.empty(shape, dtype=dtype, device=grad.device)
-        _ext._sum_by_id(grad, ids, grad_table, 0, *ctx.how)
+        _ext._sum_by_id(grad, ids, grad_table, 0, *how)
         return grad_table, None, None, None
 
 

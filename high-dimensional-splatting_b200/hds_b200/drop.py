@@ -14,15 +14,14 @@ class Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, how):
         """how: dropout()'s (p, seed, offset, rows, draw)."""
-        ctx.how = how
-        if how[-1] is not None:
-            ctx.save_for_backward(how[-1])
+        ctx.how = how[:-1]
+        ctx.save_for_backward(how[-1])
         return _ext.dropout(x, *how)
 
     @staticmethod
     def backward(ctx, grad):
-        ctx.saved_tensors  # raises if the draw has changed since
-        p, seed, offset, rows, draw = ctx.how
+        draw, = ctx.saved_tensors  # raises if it has changed since
+        p, seed, offset, rows = ctx.how
         return dropout(grad, p, seed=seed, offset=offset, rows=rows, draw=draw), None
 
 

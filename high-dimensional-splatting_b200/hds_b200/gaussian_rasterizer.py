@@ -479,20 +479,31 @@ def _draw(p, seed, offset, draw, device):
     threshold = drop_threshold(p)
     if draw is None:
         return threshold, int(seed) & _LOW64, int(offset) & _LOW64, None
+    return threshold, 0, 0, _draw_address(draw, device)
+
+
+def _draw_address(draw, device):
+    """The address of a draw tensor (None for None)."""
+    if draw is None:
+        return None
     if draw.dtype != torch.int64 or draw.shape != (2,) or not draw.is_contiguous() or draw.device != device:
         raise RuntimeError("draw must be a contiguous int64 tensor [2] (seed, offset) on the input's device")
-    return threshold, 0, 0, draw.data_ptr()
+    return draw.data_ptr()
 
 
-def _check_lookup(table_dtype, value_dtype, ids, device, padding_id):
-    if table_dtype not in _FLOATS or (value_dtype is not table_dtype and value_dtype is not _F32):
-        raise RuntimeError("the table must be float32, bfloat16 or float16, and its values of that type or float32")
+def _check_ids(ids, device):
     if ids.dtype not in _IDS:
         raise RuntimeError("ids must be an int32 or int64 tensor")
     if ids.device != device:
         raise RuntimeError("ids must be on the table's device")
     if not ids.is_contiguous():
         raise RuntimeError("ids must be contiguous")
+
+
+def _check_lookup(table_dtype, value_dtype, ids, device, padding_id):
+    if table_dtype not in _FLOATS or (value_dtype is not table_dtype and value_dtype is not _F32):
+        raise RuntimeError("the table must be float32, bfloat16 or float16, and its values of that type or float32")
+    _check_ids(ids, device)
     if padding_id is not None and not -2**63 <= padding_id < 2**63:
         raise ValueError(f"padding_id {padding_id} does not fit 64 bits")
 
@@ -534,7 +545,7 @@ def _embedding_backward(grad, ids, grad_table, accumulate, scale, padding_id, dr
 
 
 def _sum_by_id(grad, ids, grad_table, accumulate, scale, padding_id, threshold, seed, offset, draw_ptr):
-    """_embedding_backward of arguments that have been checked (autograd's: those of the forward)."""
+    """_embedding_backward of arguments that have been checked."""
     dev = grad_table.device
     v, c = grad_table.shape
     n = ids.numel()

@@ -189,3 +189,75 @@ def test_traced_calls_run_the_kernels(monkeypatch):
         traced = torch.jit.trace(f, (table,), check_trace=False)
         for t in (table, table + 1, -table):
             assert torch.equal(traced(t), want(t))
+
+
+def test_the_backward_takes_the_draw_that_was_saved(monkeypatch):
+    """Under hooks that save copies (save_on_cpu, say) the draw may move on before the backward, which then
+    has to draw the forward's mask: from the saved copy, not from where the draw was."""
+    import hds_b200
+
+    kernels = CpuKernels(monkeypatch)
+    table, ids, _ = small_lookup()
+    table.requires_grad_(True)
+    draw = torch.tensor([7, 1])
+    with torch.autograd.graph.saved_tensors_hooks(torch.clone, lambda t: t):
+        out = hds_b200.embedding(table, ids, dropout_p=0.5, draw=draw)
+        out = hds_b200.dropout(out, 0.5, draw=draw)
+    draw += 1
+    out.sum().backward()
+    assert kernels.calls == [("forward", [7, 1]), ("dropout", [7, 1]), ("dropout", [7, 1]), ("backward", [7, 1])]
+    # A draw whose memory was replaced is read where it is now: the old memory may be another tensor's.
+    out = hds_b200.embedding(table, ids, dropout_p=0.5, draw=draw)
+    draw.data = torch.tensor([9, 9])
+    out.sum().backward()
+    assert kernels.calls[-1] == ("backward", [9, 9])
+    # Without dropout the draw is not looked at: it may be anything and change.
+    draw = torch.zeros(3)
+    out = hds_b200.embedding(table, ids, draw=draw)
+    draw += 1
+    out.sum().backward()
+    assert kernels.calls[-1] == ("backward", None)
+
+
+@pytest.mark.parametrize("unpack, text", [
+    (lambda t: t.to(torch.int16), "int32 or int64"),
+    (lambda t: t[:-1], "in the forward"),
+    (lambda t: t.repeat(2), "in the forward"),
+    (lambda t: t.reshape(1, -1), "in the forward"),
+    (lambda t: t.repeat_interleave(2)[::2], "contiguous"),
+    (lambda t: t.to("meta"), "device"),
+])
+def test_the_backward_checks_the_ids_that_hooks_hand_it(monkeypatch, unpack, text):
+    """A kernel would read beyond them, or through an address of another kind."""
+    import hds_b200
+
+    kernels = CpuKernels(monkeypatch)
+    table, ids, how = small_lookup()
+    table.requires_grad_(True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        out = hds_b200.embedding(table, ids, **how)
+    with pytest.raises(RuntimeError, match=text):
+        out.sum().backward()
+    assert [c[0] for c in kernels.calls] == ["forward"]
+
+
+@pytest.mark.parametrize("unpack", [lambda t: t.int(), lambda t: t[:1], lambda t: t.to("meta"),
+                                    lambda t: t.repeat_interleave(2)[::2]])
+def test_the_backward_checks_the_draw_that_hooks_hand_it(monkeypatch, unpack):
+    import hds_b200
+
+    kernels = CpuKernels(monkeypatch)
+    table, ids, _ = small_lookup()
+    table.requires_grad_(True)
+    draw = torch.tensor([7, 1])
+
+    def changed(t):
+        return unpack(t) if t.shape == (2,) else t
+
+    for call in (lambda: hds_b200.embedding(table, ids, dropout_p=0.5, draw=draw),
+                 lambda: hds_b200.dropout(table, 0.5, draw=draw)):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, changed):
+            out = call()
+        with pytest.raises(RuntimeError, match="draw must be"):
+            out.sum().backward()
+    assert [c[0] for c in kernels.calls] == ["forward", "dropout"]

@@ -71,3 +71,23 @@ def test_forward_mode_is_refused_and_traces_run_the_kernels():
     assert torch.equal(traced(table + 1), (table + 1)[ids])
     traced = torch.jit.trace(lambda t: hds_b200.dropout(t, 0.5, seed=1), (table,), check_trace=False)
     assert torch.equal(traced(table + 1), hds_b200.dropout(table + 1, 0.5, seed=1))
+
+
+def test_saved_on_the_host_between_the_directions():
+    """save_on_cpu moves the ids and the draw to the host and back; the draw advances in between."""
+    import hds_b200
+
+    table = torch.randn(30, 16, device="cuda", requires_grad=True)
+    ids, draw = torch.arange(500, device="cuda") % 30, torch.tensor([3, 4], device="cuda")
+    grad = torch.randn(500, 16, device="cuda")
+
+    def step(**how):
+        out = hds_b200.embedding(table, ids, dropout_p=0.3, **how)
+        return hds_b200.dropout(out, 0.2, rows=True, **how)
+
+    want, = torch.autograd.grad(step(seed=3, offset=4), table, grad)
+    with torch.autograd.graph.save_on_cpu():
+        out = step(draw=draw)
+    draw += 1
+    got, = torch.autograd.grad(out, table, grad)
+    assert torch.equal(got, want)

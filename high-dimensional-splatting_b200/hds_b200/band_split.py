@@ -46,9 +46,14 @@ def band_reach_mask(means2D: torch.Tensor, radii: torch.Tensor, y0: int, y1: int
     return (radii > 0) & (v + reach >= float(y0 - 16)) & (v - reach < float(y1 + 16))
 
 
+def _kernels_take(rows: torch.Tensor) -> bool:
+    """Whether the codebook kernels take the [n, C] rows; indexing serves the rest."""
+    return rows.is_cuda and rows.shape[1] <= 32768 and rows.shape[0] <= 2**31 - 2**20
+
+
 def gather_rows(rows: torch.Tensor, ids: torch.Tensor) -> torch.Tensor:
     """rows[ids], a fresh contiguous [M, C] tensor: on the GPU the codebook lookup's kernel."""
-    if rows.is_cuda:
+    if _kernels_take(rows):
         from .gaussian_rasterizer import embedding
 
         return embedding(rows, ids.to(rows.device))
@@ -56,8 +61,11 @@ def gather_rows(rows: torch.Tensor, ids: torch.Tensor) -> torch.Tensor:
 
 
 def add_rows(target: torch.Tensor, ids: torch.Tensor, rows: torch.Tensor) -> None:
-    """target[ids] += rows: on the GPU by the codebook lookup's gradient, one pass without atomics."""
-    if target.is_cuda:
+    """target[ids] += rows: on the GPU the codebook lookup's gradient, which sorts the ids and sums without
+    atomics.  Rows of a type that promotes to target's (16-bit ones) are promoted."""
+    if torch.promote_types(rows.dtype, target.dtype) == target.dtype:
+        rows = rows.to(target.dtype)
+    if _kernels_take(target):
         from .gaussian_rasterizer import embedding_backward_into
 
         embedding_backward_into(target, rows, ids.to(target.device))

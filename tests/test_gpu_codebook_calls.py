@@ -91,3 +91,19 @@ def test_saved_on_the_host_between_the_directions():
     draw += 1
     got, = torch.autograd.grad(out, table, grad)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("c, dtype", [(40_000, torch.float32), (40_000, torch.bfloat16), (48, torch.bfloat16),
+                                      (48, torch.float16), (50, torch.int32)])
+def test_rows_of_shards_wider_than_the_kernels_take_and_of_fewer_bits(c, dtype):
+    """What the kernels do not take is indexed, and 16-bit gradients are promoted, as before them."""
+    from hds_b200.band_split import add_rows, gather_rows
+
+    table, target = torch.randn(30, c, device="cuda"), torch.randn(30, c, device="cuda")
+    ids = torch.tensor([0, 3, 4, 17, 29], device="cuda")
+    rows = (10 * torch.randn(5, c, device="cuda")).to(dtype)
+    want = target.clone()
+    want[ids] = want[ids] + rows
+    add_rows(target, ids, rows)
+    assert torch.equal(target, want)
+    assert torch.equal(gather_rows(table, ids), table[ids])

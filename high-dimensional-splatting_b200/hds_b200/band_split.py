@@ -121,17 +121,57 @@ class FeatureShards:
         self.rows.grad = torch.zeros_like(self.rows)
         self._plan = None
         self._side = None  # stream of dispatch_async
+        # 1 when this rank was asked for rows that it does not own, since the last exchange of counts.
+        self._outside = torch.zeros(1, dtype=torch.int64, device=device)
 
     def _local(self, ids: torch.Tensor) -> torch.Tensor:
         """Positions in rows of owned global ids."""
         return ids - self.start if self.owner is None else self.local_of[ids]
 
+    def _owned(self, wanted: torch.Tensor) -> torch.Tensor:
+        """_local() of the ids that a rank was asked for.  The kernels read zeros for rows outside the
+        shard, and add nothing; so they are noted, for the next exchange of counts to report."""
+        local = self._local(wanted)
+        self._outside |= ((local < 0) | (local >= self.rows.shape[0])).any()
+        return local
+
+    def check(self) -> None:
+        """Raises when this rank was asked for rows that it does not own since the last exchange of counts
+        (a host read).  Every dispatch does so on all ranks for the dispatches before it."""
+        if self._side is not None:
+            torch.cuda.current_stream(self.rows.device).wait_stream(self._side)
+        if int(self._outside):
+            self._outside.zero_()
+            raise IndexError("feature rows were asked of a rank that does not own them: the ranks' boundaries or owner "
+                             "maps differ")
+
+    def _exchange_counts(self, ids: torch.Tensor, own: torch.Tensor):
+        """Rows to send to and receive from each rank, given the requests and their owners (a host read).
+        Beside the counts travels what _owned() and these requests met outside the shards, so that all
+        ranks raise together and none waits for another in the collectives that follow."""
+        counts = torch.bincount(own, minlength=self.world)
+        if self._side is not None:  # a fetch that was never finished may still write the note
+            torch.cuda.current_stream(ids.device).wait_stream(self._side)
+        # The ids are sorted: the first may lie below the table; the owner of one beyond it is `world`.
+        outside = (self._outside + (ids[:1] < 0).sum() + counts[self.world:].sum()).expand(self.world)
+        sent = torch.stack([counts[:self.world], outside], dim=1)
+        received = torch.empty_like(sent)
+        dist.all_to_all_single(received, sent, group=self.group)
+        send, recv = sent.tolist(), received.tolist()
+        if any(flag for _, flag in recv):
+            self._outside.zero_()
+            ranks = [r for r, (_, flag) in enumerate(recv) if flag]
+            raise IndexError(f"feature rows outside the table, or of a rank that does not own them, were asked for (met by "
+                             f"ranks {ranks}): bad ids, or boundaries or owner maps that differ between the ranks")
+        return [k for k, _ in send], [k for k, _ in recv]
+
     def dispatch(self, ids: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """Rows of the sorted global ids `ids` ([M] int64), in that order ([M, C]; written into `out`
-        when given, a contiguous [M, C] tensor)."""
+        when given, a contiguous [M, C] tensor).  Ids outside the table, and rows that a dispatch before
+        this one asked of a rank that does not own them, raise IndexError on every rank."""
         if self.world == 1:
             self._plan = None
-            return gather_rows(self.rows.detach(), self._local(ids))
+            return self.rows.detach()[self._local(ids)]
         if self.owner is None:
             # Sorted ids and contiguous owners keep every owner's requests in one slice of ids.
             own = torch.searchsorted(self._bounds, ids, right=True)
@@ -140,14 +180,11 @@ class FeatureShards:
             own = self.owner[ids]
             perm = torch.argsort(own, stable=True)  # requests grouped by owner, ascending within each
             grouped = ids[perm]
-        send_counts = torch.bincount(own, minlength=self.world)
-        recv_counts = torch.empty_like(send_counts)
-        dist.all_to_all_single(recv_counts, send_counts, group=self.group)
-        send, recv = send_counts.tolist(), recv_counts.tolist()
+        send, recv = self._exchange_counts(ids, own)
         wanted = torch.empty(sum(recv), dtype=ids.dtype, device=ids.device)
         dist.all_to_all_single(wanted, grouped.contiguous(), output_split_sizes=recv, input_split_sizes=send,
                                group=self.group)
-        local = self._local(wanted)
+        local = self._owned(wanted)
         served = gather_rows(self.rows.detach(), local)
         if out is not None and perm is None:
             got = out
@@ -170,10 +207,7 @@ class FeatureShards:
             rows = self.dispatch(ids)
             return lambda: rows
         own = torch.searchsorted(self._bounds, ids, right=True)
-        send_counts = torch.bincount(own, minlength=self.world)
-        recv_counts = torch.empty_like(send_counts)
-        dist.all_to_all_single(recv_counts, send_counts, group=self.group)
-        send, recv = send_counts.tolist(), recv_counts.tolist()
+        send, recv = self._exchange_counts(ids, own)
         current = torch.cuda.current_stream(ids.device)
         if self._side is None:
             self._side = torch.cuda.Stream(ids.device)
@@ -182,7 +216,7 @@ class FeatureShards:
         with torch.cuda.stream(side):
             wanted = torch.empty(sum(recv), dtype=ids.dtype, device=ids.device)
             dist.all_to_all_single(wanted, ids, output_split_sizes=recv, input_split_sizes=send, group=self.group)
-            local = self._local(wanted)
+            local = self._owned(wanted)
             served = gather_rows(self.rows.detach(), local)
             got = torch.empty(ids.numel(), self.channels, dtype=served.dtype, device=ids.device)
             dist.all_to_all_single(got, served, output_split_sizes=send, input_split_sizes=recv, group=self.group)
@@ -201,7 +235,7 @@ class FeatureShards:
     def combine(self, ids: torch.Tensor, grads: torch.Tensor) -> None:
         """Adds grads ([M, C], rows of the ids of the last dispatch) into the owners' rows.grad."""
         if self.world == 1:
-            add_rows(self.rows.grad, self._local(ids), grads.contiguous())
+            self.rows.grad.index_add_(0, self._local(ids), grads)
             return
         send, recv, local, perm = self._plan
         outgoing = grads if perm is None else grads[perm]

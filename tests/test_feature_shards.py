@@ -85,3 +85,74 @@ def test_gradients_of_fewer_bits_are_promoted():
     for dtype in ("torch.float32", "torch.bfloat16", "torch.float16", "torch.int32"):
         assert torch.equal(torch.tensor(ranks[0][dtype] + ranks[1][dtype]), want), dtype
     assert ranks[0]["float64"] == ranks[1]["float64"] == "refused"
+
+
+def _raises(call):
+    try:
+        call()
+    except IndexError as err:
+        return str(err)
+    return None
+
+
+def _bad_ids(rank):
+    """Rank 1 asks for ids outside the table; rank 0's are good.  Both raise, and go on afterwards."""
+    from hds_b200.band_split import FeatureShards
+
+    shards = FeatureShards(10, 8, rank, WORLD, "cpu", init=table_rows)
+    out = []
+    for bad in ([2, 10], [2, 2**40], [-1, 3]):
+        ids = torch.tensor([1, 6] if rank == 0 else bad)
+        out.append(_raises(lambda: shards.dispatch(ids)))
+        good = torch.tensor([rank, 5 + rank])
+        out.append(torch.equal(shards.dispatch(good), table_rows(0, 10)[good]))
+        empty = shards.dispatch(good[:0] if rank else good)
+        out.append(tuple(empty.shape) == ((0, 8) if rank else (2, 8)))
+    out.append(_raises(shards.check))
+    return out
+
+
+def test_ids_outside_the_table_raise_on_every_rank():
+    for result in on_two_ranks(_bad_ids):
+        for error, again, empty in zip(result[0:9:3], result[1:9:3], result[2:9:3]):
+            assert "outside the table" in error and "[1]" in error
+            assert again and empty
+        assert result[9] is None
+
+
+def _different_boundaries(rank):
+    """Rank 0 takes rank 1's rows to begin at 5, rank 1 at 6: row 5 has no owner."""
+    from hds_b200.band_split import FeatureShards
+
+    shards = FeatureShards(10, 8, rank, WORLD, "cpu", init=table_rows, starts=[0, 5 + rank, 10])
+    good = torch.tensor([1, 7])
+    out = [_raises(lambda: shards.dispatch(good)) is None]
+    shards.dispatch(torch.tensor([5]) if rank == 0 else good)  # met by rank 1, which has no such row
+    out.append(_raises(lambda: shards.dispatch(good)))
+    out.append(_raises(lambda: shards.dispatch(good)) is None)
+    shards.dispatch(torch.tensor([5]) if rank == 0 else good)
+    out.append(_raises(shards.check))
+    return out
+
+
+def test_rows_asked_of_a_rank_that_does_not_own_them_are_reported():
+    for rank, (first, error, later, checked) in enumerate(on_two_ranks(_different_boundaries)):
+        assert first and later
+        assert "differ between the ranks" in error and "[1]" in error
+        assert (checked is not None) == (rank == 1)
+
+
+def test_one_rank_indexes_its_rows():
+    """Ids that are no rows raise at once on the CPU; gradients of another type are refused."""
+    from hds_b200.band_split import FeatureShards
+
+    shards = FeatureShards(10, 8, 0, 1, "cpu", init=table_rows)
+    ids = torch.tensor([1, 4, 9])
+    assert torch.equal(shards.dispatch(ids), table_rows(0, 10)[ids])
+    for _ in range(2):
+        shards.combine(ids, torch.ones(8, 3).T)
+    want = torch.zeros(10, 8)
+    want[ids] = 2
+    assert torch.equal(shards.rows.grad, want)
+    with pytest.raises(IndexError):
+        shards.dispatch(torch.tensor([10]))

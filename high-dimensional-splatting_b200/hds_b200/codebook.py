@@ -11,6 +11,7 @@ import torch
 
 from . import gaussian_rasterizer as _ext
 from . import rasterizer
+from .drop import draw_numbers
 
 
 class Embedding(torch.autograd.Function):
@@ -57,8 +58,8 @@ class Embedding(torch.autograd.Function):
 
 
 def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, padding_id: int | None = None,
-              dtype: torch.dtype | None = None, dropout_p: float = 0.0, seed: int = 0, offset: int = 0,
-              draw: torch.Tensor | None = None) -> torch.Tensor:
+              dtype: torch.dtype | None = None, dropout_p: float = 0.0, seed: int | None = None,
+              offset: int | None = None, draw: torch.Tensor | None = None) -> torch.Tensor:
     """scale * table[ids]: the features [*ids.shape, C] of the codeword ids under the codebook table
     [V, C] (float32, bfloat16 or float16; ids int32 or int64), in `dtype` (the table's type, or float32:
     the type rasterize takes).  Differentiable in table; the same backward call gives the same bits.
@@ -68,14 +69,16 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, pad
     zeros and no gradient.  Any other id outside [0, V) does too, and sets native.device_status().
 
     dropout_p: drops elements of the result with this probability (a multiple of 1/65536) and scales the
-    others up, in the same pass.  The mask follows from (seed, offset) -- a step counter, say, as the
-    offset -- and is drawn anew in the backward, never stored.  draw: an int64 tensor [2] = (seed, offset)
+    others up, in the same pass.  The mask follows from (seed, offset) alone (0 when not given; a call that
+    gives neither, nor draw, warns): give every step and use its own, a step counter, say, as the offset.
+    It is drawn anew in the backward, never stored.  draw: an int64 tensor [2] = (seed, offset)
     on the device, used instead of the two numbers and read when the kernels run, so that a captured
     graph can advance it; it must not change between a forward and its backward.
 
     To capture a backward pass into a CUDA graph, keep no eager autograd graph of the same table alive
     (torch ties the leaf's gradient to the stream of the first one); gaussian_rasterizer.embedding_backward
     has no such rule."""
+    seed, offset = draw_numbers(dropout_p, seed, offset, draw)
     table = table.contiguous()
     ids = ids.contiguous()
     if rasterizer.needs_node(table):

@@ -261,3 +261,28 @@ def test_the_backward_checks_the_draw_that_hooks_hand_it(monkeypatch, unpack):
         with pytest.raises(RuntimeError, match="draw must be"):
             out.sum().backward()
     assert [c[0] for c in kernels.calls] == ["forward", "dropout"]
+
+
+def test_a_mask_that_depends_on_nothing_given_warns(monkeypatch):
+    """Without seed, offset or draw every call and layer would drop the same elements."""
+    import warnings
+
+    import hds_b200
+
+    CpuKernels(monkeypatch)
+    table, ids, _ = small_lookup()
+    with pytest.warns(UserWarning, match="same at every call"):
+        hds_b200.dropout(table, 0.5)
+    with pytest.warns(UserWarning, match="same at every call") as seen:
+        hds_b200.embedding(table, ids, dropout_p=0.5)
+    assert seen[0].filename == __file__
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        for how in (dict(seed=0), dict(offset=0), dict(seed=3, offset=4), dict(draw=torch.tensor([1, 2]))):
+            hds_b200.dropout(table, 0.5, **how)
+            hds_b200.embedding(table, ids, dropout_p=0.5, **how)
+            leaf = table.clone().requires_grad_(True)
+            hds_b200.dropout(hds_b200.embedding(leaf, ids, dropout_p=0.5, **how), 0.5, **how).sum().backward()
+        for p in (0.0, 1.0):  # nothing is drawn, or nothing depends on it
+            hds_b200.dropout(table, p)
+            hds_b200.embedding(table, ids, dropout_p=p)

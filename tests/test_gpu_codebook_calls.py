@@ -107,3 +107,51 @@ def test_rows_of_shards_wider_than_the_kernels_take_and_of_fewer_bits(c, dtype):
     add_rows(target, ids, rows)
     assert torch.equal(target, want)
     assert torch.equal(gather_rows(table, ids), table[ids])
+
+
+@pytest.mark.parametrize("n", [100, 6000, 100_000])  # one launch; the sort in one digit and some tiles; in many
+@pytest.mark.parametrize("c", [24, 13])
+@pytest.mark.parametrize("p", [0.0, 0.4])
+@pytest.mark.parametrize("padding_id, vocab", [(-1, 40), (7, 40), (2999, 3000)])  # outside and inside the table
+def test_nothing_but_padding(n, c, p, padding_id, vocab):
+    """No row to look up or to sum, at the sizes of every form: values and gradient are zeros whatever the
+    table and the incoming gradient hold, and a buffer that is added to keeps its bits."""
+    import hds_b200
+    from hds_b200 import gaussian_rasterizer as ext
+    from hds_b200 import native
+
+    table = torch.full((vocab, c), float("nan"), device="cuda", requires_grad=True)
+    ids = torch.full((n,), padding_id, device="cuda")
+    how = dict(padding_id=padding_id, dropout_p=p, seed=1, offset=2)
+    out = hds_b200.embedding(table, ids, **how)
+    assert torch.equal(out.detach(), torch.zeros(n, c, device="cuda"))
+    grad = torch.full_like(out, float("inf"))
+    got, = torch.autograd.grad(out, table, grad)
+    assert torch.equal(got, torch.zeros(vocab, c, device="cuda"))
+    before = torch.randn(vocab, c, device="cuda")
+    before[0, 0], before[-1, -1] = float("nan"), -0.0
+    buffer = before.clone()
+    ext.embedding_backward_into(buffer, grad.detach(), ids, **how)
+    assert torch.equal(buffer.view(torch.int32), before.view(torch.int32))
+    assert native.device_status() == 0
+
+
+@pytest.mark.parametrize("n", [100, 6000, 100_000])
+@pytest.mark.parametrize("c", [24, 13])
+def test_one_row_among_padding(n, c):
+    """All rows but the last are padding, at the sizes of every form."""
+    from hds_b200 import gaussian_rasterizer as ext
+
+    ids = torch.full((n,), -1, device="cuda")
+    ids[-1] = 39
+    grad = torch.full((n, c), float("nan"), device="cuda")
+    grad[-1] = torch.randn(c, device="cuda")
+    got = ext.embedding_backward(grad, ids, 40, padding_id=-1)
+    want = torch.zeros(40, c, device="cuda")
+    want[39] = grad[-1]
+    assert torch.equal(got, want)
+    table = torch.full((40, c), float("nan"), device="cuda")
+    table[39] = torch.randn(c, device="cuda")
+    values = torch.zeros(n, c, device="cuda")
+    values[-1] = table[39]
+    assert torch.equal(ext.embedding(table, ids, padding_id=-1), values)

@@ -7,15 +7,30 @@ from __future__ import annotations
 
 import math
 import multiprocessing.util
+import threading
 import time
+from multiprocessing import resource_sharer
 
 import numpy as np
 
-# A spawned worker that sends tensors through a queue serves their file descriptors until it exits; the
-# parent may still be fetching them then.  A worker that imports this module stays a moment longer, before
-# its exit closes the socket they are fetched through (priority 0).
+
+def _stay_until_fetched():
+    """A spawned worker that sends tensors through a queue serves their file descriptors until it exits; the
+    parent may still be fetching them then.  A worker that imports this module first lets the queues'
+    threads send what they hold, then waits until every descriptor has been fetched (30 s at most)."""
+    end = time.monotonic() + 30.0
+    for thread in threading.enumerate():
+        if thread.name == "QueueFeederThread":
+            thread.join(max(0.0, end - time.monotonic()))
+    while resource_sharer._resource_sharer._cache and time.monotonic() < end:
+        time.sleep(0.01)
+    resource_sharer.stop(timeout=5.0)  # joins the thread that hands them over
+
+
+# After the queues have been told to close (priority 10), before the socket closes that the descriptors are
+# fetched through (0).
 if multiprocessing.current_process().name != "MainProcess":
-    multiprocessing.util.Finalize(None, time.sleep, args=(1.0,), exitpriority=100)
+    multiprocessing.util.Finalize(None, _stay_until_fetched, exitpriority=5)
 
 # Tolerances from the build's north star: RGB within 1e-5 absolute, feature images within 1e-3
 # absolute, gradients within 1e-4 relative (every entry within 1e-4 of the tensor's largest

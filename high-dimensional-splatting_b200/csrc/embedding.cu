@@ -450,13 +450,15 @@ __global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(int n, PairSource
 constexpr int COLUMNS = 8;       // per lane
 constexpr int ROWS_AHEAD = 4;    // rows loaded before the first is added
 
+// The sum of no rows is stored as +0 whatever the factor's sign (the addition of 0 turns -0 into it), as the
+// memset of the sorted form leaves it.
 template <typename T, int V, bool ACCUMULATE>
 __device__ __forceinline__ void store_sum(T* p, const float* sum, float factor) {
     Vec<T, V> old;
     if (ACCUMULATE) old = load_once<T, V>(p);
     float r[V];
 #pragma unroll
-    for (int j = 0; j < V; j++) r[j] = ACCUMULATE ? fmaf(factor, sum[j], old.get(j)) : factor * sum[j];
+    for (int j = 0; j < V; j++) r[j] = fmaf(factor, sum[j], ACCUMULATE ? old.get(j) : 0.0f);
     store<T, V>(p, Vec<T, V>::pack(r));
 }
 
@@ -832,18 +834,9 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(int n, int channe
                 store_sum<T, V, ACCUMULATE>(table + (int64_t)(first + codeword) * channels + c0 + column(k),
                                             sum + k * V, factor);
     };
-    const auto clear = [&](int codeword) {  // +0, as the memset of the sorted form leaves it
-#pragma unroll
-        for (int k = 0; k < STEPS; k++)
-            if (column(k) < width)
-                store<T, V>(table + (int64_t)(first + codeword) * channels + c0 + column(k), Vec<T, V>{});
-    };
     for (int v = worker; v < here; v += workers) {
         const uint32_t from = s_start[v], to = s_start[v + 1];
-        if (from == to) {
-            if (!ACCUMULATE) clear(v);
-            continue;
-        }
+        if (ACCUMULATE && from == to) continue;
         if (to - from > SHORT_ROWS) {
             if (lane == 0) s_long_codeword[atomicAdd(&s_long, 1)] = (uint16_t)v;
             continue;

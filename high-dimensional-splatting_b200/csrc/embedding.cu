@@ -3,8 +3,9 @@
 // elements in the same pass (philox.cuh): f = scale / kept share, dropped elements 0 in both directions.
 //
 // Lookup.  One pass: the output is written once, the table's rows come from the L2 when the codebook is
-// smaller than it.  Bound by the writes: 1.18M x 512 fp32 in 400 us, 2.4 GB at 6.1 TB/s (0.93 of the measured
-// copy rate); with dropout 424 us, where the generator's integer work begins to count.
+// smaller than it.  Bound by the writes: 1.18M x 512 fp32 in 400 to 414 us alone, 2.4 GB at 5.9 to 6.1 TB/s
+// (0.90 to 0.93 of the measured copy rate), 444 to 449 us (0.83 to 0.84) in passes over changing inputs;
+// with dropout 424 to 442 us alone, where the generator's integer work begins to count.
 //
 // Gradient.  The rows are put in codeword order by a stable radix sort of (id, row number), and each
 // codeword's rows are summed in that order in fp32: no float atomics, so a call's result does not depend
@@ -131,7 +132,10 @@ __global__ void __launch_bounds__(THREADS, DROP ? 8 : 1)
 // Eight rows are whole groups, so a block takes `eights` times eight rows, group by group: one generator
 // call still serves eight elements, an id eight of its row's, and the output is one vector.  A group's elements
 // come from the table in vectors of V, from two rows at most (any number when rows are narrower than a
-// group).  (With a thread per element 1.18M x 75 fp32 took 174 us, 109 like this.)
+// group).  (With a thread per element 1.18M x 75 fp32 took 174 us, 108 like this.)  With scalar loads the L1's
+// rate bounds it (98% of its peak at 1.18M x 75 fp32, twice the bytes' floor of 55 us); with dropout in
+// 16 bits the integer work (74% of the issue slots, 19% of the memory's rate: 102 us for 1M x 100 bf16,
+// floor 33 us).
 template <typename T, typename O, int V, bool DROP>
 __global__ void __launch_bounds__(THREADS) lookup_groups_kernel(int n, int channels, int eights, Divider rows_of,
                                                                 const T* __restrict__ table, Ids ids, float factor,
@@ -445,8 +449,10 @@ __global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(int n, PairSource
 // group of 1 to 32 lanes with 8 columns each, adds up one chunk's rows in registers.  A codeword that
 // begins and ends inside the chunk goes straight to the table.  The sum of a codeword that began in an
 // earlier chunk is the chunk's head, that of one that goes on into the next its tail; join_kernel adds a
-// tail and the heads that follow it.  Bound by the memory: 1.18M x 512 fp32 rows are read at 6.1 TB/s, 0.94
-// of the measured copy rate; with dropout by the generator's integer work.
+// tail and the heads that follow it.  Bound by the memory: fp32 rows of 512 columns are read at 6.2 TB/s, 0.94
+// of the measured copy rate, rows of 128 at 5.9.  With dropout nothing is full (58% of the issue slots, 61% of
+// the memory's rate): the generator and the loads take turns in the 30% of the warps that fit.  Odd widths
+// load scalars and wait for them (1.18M x 75 fp32: 154 us, 37% of the memory's rate, 24% of the warps).
 constexpr int COLUMNS = 8;       // per lane
 constexpr int ROWS_AHEAD = 4;    // rows loaded before the first is added
 
@@ -691,10 +697,18 @@ __global__ void __launch_bounds__(THREADS) join_kernel(int64_t n, uint32_t vocab
 // the rows whose codeword is its own, groups them by codeword in shared memory (the scatter's ranking:
 // row order stays), adds each codeword's rows and writes every row of its range, zeros included.  Each
 // block reads all the ids, which is cheap while there are few; in return nothing waits for a second
-// launch.  Measured with events around the call: 4096 x 32 rows of 256 codewords 18 us, 29 with the sort; 300 x 64
-// of 1000 12 and 28; 4096 x 512 of 256 37 and 31, where the six launches saved on the host still count; at
-// 8192 x 512 57 and 35.  A worker of 1 to FEW_LANES lanes (8 columns each) adds the rows of a codeword; one
-// with many rows is added by the whole block, every worker a run of interleaved rows, and a tree.
+// launch.  A worker of 1 to FEW_LANES lanes (8 columns each) adds the rows of a codeword; one with many rows
+// is added by the whole block, every worker a run of interleaved rows, and a tree.
+//
+// Measured against the sorted form, us a call, called in a loop / replayed from a captured graph:
+//   4096 x 32 of 256      11.5 / 10.3   sorted 24.8 / 16.4        300 x 64 of 1000   11.5 / 10.3   24.0 / 16.4
+//   4096 x 512 of 256     18.5 / 18.4          24.1 / 17.7        4096 x 1000 of 4096  22.6 / 22.6  39.0 / 26.7
+//   4096 x 75 of 256      24.6 / 24.6          25.7 / 20.5        8192 x 512: 57 us with events around it, 35 sorted
+// so up to 4096 rows it is ahead in a loop (the sorted form's launches cost the host) and level or ahead in
+// a graph but for odd widths.  With dropout at odd widths it is not: its decisions for 8 scalar columns of 4
+// rows spill (128 registers), and from about 512 rows on it falls behind (4096 x 75 of 256: 54.4 / 53.7 and
+// 25.7 / 20.5; 4096 x 501: 117 and 29).  It is taken there all the same: the caller's scratch follows from the
+// sizes alone, which tell neither dropout nor alignment.
 constexpr int FEW_THREADS = 512;
 constexpr int FEW_ROUNDS = 8;                        // ids per thread
 constexpr int FEW_ROWS = FEW_THREADS * FEW_ROUNDS;  // 4096

@@ -19,7 +19,8 @@ class Embedding(torch.autograd.Function):
 
     Under hds_b200.rasterizer.accumulate_leaf_grads() (active during this forward), when table is a leaf
     that already holds a contiguous float32 .grad of its shape, the backward adds into that buffer and
-    hands autograd no gradient for it (hooks on the table do not see that gradient)."""
+    hands autograd no gradient for it (hooks on the table do not see that gradient; forwards that share the
+    table then belong on one stream)."""
 
     @staticmethod
     def forward(ctx, table, ids, dtype, how):

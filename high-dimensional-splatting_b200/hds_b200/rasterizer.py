@@ -35,7 +35,9 @@ def _fused_backward(channels: int) -> bool:
 # autograd no gradient for it), instead of returning a fresh [N, D] tensor that autograd then adds.
 # hds_b200.sh.eval_sh_grad does the same for sh_dc and sh_rest.  The flag is read when the forward
 # runs.  For loops that accumulate several views into one gradient buffer.  Hooks registered on
-# those tensors are not run for that gradient.  Off by default (the reference's behaviour).
+# those tensors are not run for that gradient.  A backward pass runs on its forward's stream, and the adds
+# of two streams into one buffer are not ordered: keep the forwards that share a leaf on one stream.
+# Off by default (the reference's behaviour).
 ACCUMULATE_INTO_LEAF_GRAD: bool = False
 
 

@@ -32,7 +32,7 @@ def _stay_until_fetched():
 if multiprocessing.current_process().name != "MainProcess":
     multiprocessing.util.Finalize(None, _stay_until_fetched, exitpriority=5)
 
-# Tolerances from the build's north star: RGB within 1e-5 absolute, feature images within 1e-3
+# Tolerances: RGB within 1e-5 absolute, feature images within 1e-3
 # absolute, gradients within 1e-4 relative (every entry within 1e-4 of the tensor's largest
 # reference entry).
 RGB_ATOL = 1e-5
@@ -81,7 +81,7 @@ def grad_rel_error(got, want) -> float:
 
 
 def assert_grads_close(got, want, what: str = "", rel: float = GRAD_REL) -> None:
-    """|got - want| <= rel * max|want| for every entry: the north star's 1e-4 relative bound on FP32
+    """|got - want| <= rel * max|want| for every entry: the 1e-4 relative bound on FP32
     gradients, relative to the tensor's largest entry (entries sum float atomics in any order, so
     single small entries carry the rounding of large ones).  Records the worst relative error."""
     got = np.asarray(got, np.float64)

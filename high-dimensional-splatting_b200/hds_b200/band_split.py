@@ -161,8 +161,8 @@ class FeatureShards:
         if any(flag for _, flag in recv):
             self._outside.zero_()
             ranks = [r for r, (_, flag) in enumerate(recv) if flag]
-            raise IndexError(f"feature rows outside the table, or of a rank that does not own them, were asked for (met by "
-                             f"ranks {ranks}): bad ids, or boundaries or owner maps that differ between the ranks")
+            raise IndexError(f"feature rows outside the table, or of a rank that does not own them, were asked for (met "
+                             f"by ranks {ranks}): bad ids, or boundaries or owner maps that differ between the ranks")
         return [k for k, _ in send], [k for k, _ in recv]
 
     def dispatch(self, ids: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:

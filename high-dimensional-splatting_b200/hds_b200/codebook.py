@@ -72,9 +72,9 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, pad
     dropout_p: drops elements of the result with this probability (a multiple of 1/65536) and scales the
     others up, in the same pass.  The mask follows from (seed, offset) alone (0 when not given; a call that
     gives neither, nor draw, warns): give every step and use its own, a step counter, say, as the offset.
-    It is drawn anew in the backward, never stored.  draw: an int64 tensor [2] = (seed, offset)
-    on the device, used instead of the two numbers and read when the kernels run, so that a captured
-    graph can advance it; it must not change between a forward and its backward.
+    It is drawn anew in the backward, never stored.  draw: an int64 tensor [2] = (seed, offset) on the
+    device, used instead of the two numbers and read when the kernels run, so that a captured graph can
+    advance it; it must not change between a forward and its backward.
 
     To capture a backward pass into a CUDA graph, keep no eager autograd graph of the same table alive
     (torch ties the leaf's gradient to the stream of the first one); gaussian_rasterizer.embedding_backward

@@ -30,8 +30,8 @@ class Dropout(torch.autograd.Function):
 def draw_numbers(p: float, seed: int | None, offset: int | None, draw: torch.Tensor | None) -> tuple[int, int]:
     """(seed, offset), 0 for those not given; warns when a mask would depend on nothing that was given."""
     if seed is None and offset is None and draw is None and 0 < p < 1:
-        warnings.warn("dropout without seed, offset or draw takes the mask of (0, 0): the same at every call and in every "
-                      "layer", stacklevel=3)
+        warnings.warn("dropout without seed, offset or draw takes the mask of (0, 0): the same at every call and in "
+                      "every layer", stacklevel=3)
     return seed or 0, offset or 0
 
 
@@ -43,9 +43,9 @@ def dropout(x: torch.Tensor, p: float, *, seed: int | None = None, offset: int |
 
     The mask follows from (seed, offset) alone, which are 0 when not given: give every step and every use
     numbers of its own (a step counter as the offset, say), or they all drop the same elements.  A call
-    that gives neither, nor draw, warns.  draw: an int64 tensor [2] = (seed, offset) on the device, used instead of the two numbers and read when the
-    kernel runs, so that a captured graph can advance it; it must not change between a forward and its
-    backward.  A p that rounds to 0 returns x itself."""
+    that gives neither, nor draw, warns.  draw: an int64 tensor [2] = (seed, offset) on the device, used instead
+    of the two numbers and read when the kernel runs, so that a captured graph can advance it; it must not
+    change between a forward and its backward.  A p that rounds to 0 returns x itself."""
     if _ext.drop_threshold(p) == 0:
         return x
     seed, offset = draw_numbers(p, seed, offset, draw)

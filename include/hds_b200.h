@@ -321,9 +321,9 @@ int hds_densify_apply(int n_old, int n_new, int segments, const int* widths, int
  * graph can take a new mask at every replay.  Dropped elements are 0 whatever the input holds.
  *
  * hds_embedding_forward: out[i] = scale * table[ids[i]] [n, channels]; scale * 65536 / (65536 - T) must be
- * finite in fp32, in both directions.  An id equal to padding_id (when
- * has_padding) gives a row of zeros and takes no gradient.  So does any other id outside [0, vocab),
- * which also records HDS_ERR_INVALID in the device status (hds_device_status).
+ * finite in fp32, in both directions.  An id equal to padding_id (when has_padding) gives a row of zeros
+ * and takes no gradient.  So does any other id outside [0, vocab), which also records HDS_ERR_INVALID in
+ * the device status (hds_device_status).
  *
  * hds_embedding_backward: grad_table[v] = scale * sum of grad[i] over the i with ids[i] = v, in fp32 and
  * in an order that depends on the arguments alone: the same call gives the same bits.  accumulate != 0
@@ -355,8 +355,8 @@ int hds_embedding_backward(int64_t n, int64_t vocab, int64_t channels, int grad_
 int hds_dropout(int64_t rows, int64_t channels, int type, const void* x, int drop_threshold, int whole_rows,
                 uint64_t seed, uint64_t offset, const int64_t* draw, void* y, hds_stream_t stream);
 
-/* Reads and clears the device-side failure word that kernels with bounded waits and the codebook lookup
- * set (0 = none).  Synchronises `stream`. */
+/* Reads and clears the failure word of the current device, which kernels with bounded waits and the codebook
+ * lookup set (0 = none).  Synchronises `stream`, one of that device. */
 int hds_device_status(int* status, hds_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------

@@ -155,3 +155,25 @@ def test_one_row_among_padding(n, c):
     values = torch.zeros(n, c, device="cuda")
     values[-1] = table[39]
     assert torch.equal(ext.embedding(table, ids, padding_id=-1), values)
+
+
+@pytest.mark.parametrize("n, c", [(500, 24), (20_000, 24), (20_000, 13)])
+def test_adding_into_the_leaf_on_a_side_stream_is_done_when_the_backward_returns(n, c):
+    """The add is all that the backward leaves behind (autograd gets no gradient): the caller's stream has to
+    wait for it all the same, and for what went before it on the side stream (here a pause)."""
+    import hds_b200
+
+    table = torch.randn(50, c, device="cuda", requires_grad=True)
+    ids, grad = torch.arange(n, device="cuda") % 50, torch.randn(n, c, device="cuda")
+    table.grad = torch.zeros_like(table)
+    want, = torch.autograd.grad(hds_b200.embedding(table, ids), table, grad)
+    side = torch.cuda.Stream()
+    for k in range(1, 4):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side), hds_b200.accumulate_leaf_grads():
+            torch.cuda._sleep(20_000_000)
+            out = hds_b200.embedding(table, ids)
+            out.record_stream(torch.cuda.current_stream())
+        out.backward(grad)
+        seen = table.grad.clone()
+        assert torch.allclose(seen, k * want, rtol=1e-5, atol=1e-5 * float(want.abs().max()))
